@@ -16,6 +16,10 @@ CIRCUIT_BATCH_MAX_K = 256
 CIRCUIT_BATCH_MAX_DIM = 2048
 CIRCUIT_MAX_RANK = 64
 CIRCUIT_MAX_DIM = 2048
+CIRCUIT_INT8_MAX_DIM = 16384
+CIRCUIT_INT8_MAX_QUERIES = 65535
+CIRCUIT_F32, CIRCUIT_F16, CIRCUIT_BF16 = 0, 1, 2
+CIRCUIT_NORM_NONE, CIRCUIT_NORM_RMS, CIRCUIT_NORM_UNIT = 0, 1, 2
 TRACE_SNAPSHOT_BYTES = 96
 
 # every symbol declared in include/circuit.h and include/circuit_ops.h
@@ -38,6 +42,9 @@ EXPORTED_SYMBOLS = (
     "circuit_op_score_surviving_leaves",
     "circuit_op_flat_exact_score",
     "circuit_op_hierarchical_search",
+    "circuit_op_quantize_rows",
+    "circuit_op_dequantize_rows",
+    "circuit_op_int8_scores",
     "circuit_merge_topk",
     "circuit_merge_topk_batch",
     "circuit_plan_shards",
@@ -116,6 +123,10 @@ def _declare(lib):
         "circuit_op_score_surviving_leaves": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I, _P, _P]),
         "circuit_op_flat_exact_score": (_I, [_P, _P, _I64, _I, _P, _P]),
         "circuit_op_hierarchical_search": (_I, [_P] * 21 + [_I, _I, _I64, _I, _F, _I, _F, _P]),
+        "circuit_op_quantize_rows": (_I, [_P, _I, _I64, _I, _I64, _P, _I64, _P, _I, _I, _F, _P, _I64, _P, _I, _I64, _P,
+                                          _I64, _P, _P]),
+        "circuit_op_dequantize_rows": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I64, _P, _I, _I64, _P]),
+        "circuit_op_int8_scores": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _P, _P, _I, _I64, _P]),
         "circuit_merge_topk": (_I, [_P, _P, _I, _I, _P, _P, _P]),
         "circuit_merge_topk_batch": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
         "circuit_plan_shards": (_I, [_P, _I, _I, _P, _P]),

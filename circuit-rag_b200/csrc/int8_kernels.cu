@@ -1,0 +1,626 @@
+// Rows in 8 bits (include/circuit_ops.h, the int8 section): quantisation with
+// one scale a row (plain, after a root-mean-square norm with the residual's
+// addition, or to unit length; into consecutive rows or into the slots of a row
+// store), reading rows back by id, and products of 8-bit queries with 8-bit rows.
+//
+// Mathematics.  With v = x (+ residual, rounded once to the row's type) and
+// u = v * w, a row's codes are rint(127 u_j / a), a = max|u|, and its scale is
+// a / 127 times the norm's factor.  The norm's factor cancels in the codes, so
+// they depend on no sum and are the same whatever its order: k_quantize_rows
+// gives the correctly rounded code of the real quotient (see code_of), and only
+// the scale carries the rounding of the 32-bit sum of squares.
+#include <cfloat>
+#include <cstdint>
+#include <string>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/circuit_ops.h"
+#include "common.cuh"
+#include "index_internal.h"
+
+namespace cb {
+namespace i8 {
+
+// ---------------------------------------------------------------- row types
+template <typename T>
+struct RowType;  // V: elements of a 16-byte vector
+template <>
+struct RowType<float> {
+  static constexpr int V = 4;
+  __device__ static float get(float x) { return x; }
+  __device__ static float put(float x) { return x; }
+};
+template <>
+struct RowType<__half> {
+  static constexpr int V = 8;
+  __device__ static float get(__half x) { return __half2float(x); }
+  __device__ static __half put(float x) { return __float2half_rn(x); }
+};
+template <>
+struct RowType<__nv_bfloat16> {
+  static constexpr int V = 8;
+  __device__ static float get(__nv_bfloat16 x) { return __bfloat162float(x); }
+  __device__ static __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
+};
+
+template <typename T>
+union Vec {
+  uint4 raw;
+  T e[RowType<T>::V];
+};
+
+// Elements [c, c + V) of a row of d elements: one 16-byte access where the row
+// allows it, else one access an element; zeros past the row's end.
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* row, int c, int d, bool wide) {
+  constexpr int V = RowType<T>::V;
+  Vec<T> v;
+  v.raw = make_uint4(0, 0, 0, 0);
+  if (wide && c + V <= d) {
+    v.raw = *reinterpret_cast<const uint4*>(row + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i < d) v.e[i] = row[c + i];
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* row, int c, int d, bool wide, const Vec<T>& v) {
+  constexpr int V = RowType<T>::V;
+  if (wide && c + V <= d) {
+    *reinterpret_cast<uint4*>(row + c) = v.raw;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c + i < d) row[c + i] = v.e[i];
+  }
+}
+
+// ---------------------------------------------------------------- reductions over the G threads of a row
+struct RowSums {
+  float top, low;  // max |u| as the unevaluated sum top + low (top = the rounded product)
+  float ss;        // sum of v^2
+  int bad;         // some u is not finite
+};
+// (top, low) of two candidates: the larger real number.
+__device__ __forceinline__ void raise(float& top, float& low, float t, float l) {
+  if (t > top || (t == top && l > low)) {
+    top = t;
+    low = l;
+  }
+}
+template <int G>
+__device__ __forceinline__ RowSums reduce(RowSums r) {
+  constexpr int W = G < 32 ? G : 32;
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    const float t = __shfl_xor_sync(FULL_MASK, r.top, o), l = __shfl_xor_sync(FULL_MASK, r.low, o);
+    raise(r.top, r.low, t, l);
+    r.ss += __shfl_xor_sync(FULL_MASK, r.ss, o);
+    r.bad |= __shfl_xor_sync(FULL_MASK, r.bad, o);
+  }
+  if constexpr (G > 32) {
+    __shared__ RowSums part[G / 32];
+    __syncthreads();  // the previous call's readers are done
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = r;
+    __syncthreads();
+    r = part[0];
+#pragma unroll
+    for (int w = 1; w < G / 32; ++w) {
+      raise(r.top, r.low, part[w].top, part[w].low);
+      r.ss += part[w].ss;
+      r.bad |= part[w].bad;
+    }
+  }
+  return r;
+}
+
+// The code of u = v * w: rint(127 u / a) of the real quotient, ties to even.
+// t = u * (127 / a) in 32 bits is within 3.1e-5 of 127 u / a (four roundings of
+// relative size 2^-24 at |t| <= 127), so its nearest integer is the code unless
+// t lies within 6e-5 of a half; there (0.012 % of the values) the quotient is
+// taken in 64 bits, where v * w is exact.
+constexpr float NEAR_HALF = 0.5f - 6e-5f;
+__device__ __forceinline__ int code_near_half(float v, float w, double a) {
+  return (int)rint((double)v * (double)w * 127.0 / a);
+}
+
+struct QuantizeParams {
+  const void* x;
+  const void* res;      // nullptr: no residual
+  const void* w;        // nullptr: no weight
+  void* sum;            // x + res, written when res is given
+  const void* slots;    // nullptr: row i to row i
+  int8_t* codes;
+  float* scales;
+  int64_t n, x_stride, res_stride, sum_stride, code_stride, capacity;
+  int d;
+  int w_f32;            // the weight is fp32 (else of the row's type)
+  int norm;             // 0: scale a / 127; else divided by sqrt(ss * inv_n + eps)
+  float inv_n, eps;
+  int slot64, claimed;  // slots are int64; slots were claimed by k_claim_slots
+  int wide_in, wide_out;
+};
+
+__device__ __forceinline__ int64_t slot_at(const void* slots, int slot64, int64_t i) {
+  return slot64 ? reinterpret_cast<const long long*>(slots)[i] : (int64_t) reinterpret_cast<const int*>(slots)[i];
+}
+// A slot's claim by row i of a write: above every scale's bit pattern (scales
+// are never negative), larger for later rows.
+__device__ __forceinline__ uint32_t claim_tag(int64_t i) { return 0x80000000u | (uint32_t)i; }
+
+__global__ void k_reset_slots(const void* slots, int slot64, int64_t n, int64_t capacity, float* scales) {
+  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int64_t s = slot_at(slots, slot64, i);
+  if (s >= 0 && s < capacity) scales[s] = 0.f;
+}
+__global__ void k_claim_slots(const void* slots, int slot64, int64_t n, int64_t capacity, float* scales) {
+  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int64_t s = slot_at(slots, slot64, i);
+  if (s >= 0 && s < capacity) atomicMax(reinterpret_cast<uint32_t*>(scales + s), claim_tag(i));
+}
+
+// G threads a row (a warp, or a block of G), the row in NV 16-byte vectors of
+// registers a thread: it is read once and never again.  FULL: with residual,
+// weight and norm as the parameters say; otherwise the plain quantisation.
+constexpr int quantize_threads(int G) { return G == 32 ? 256 : G; }
+
+template <typename T, int G, int NV, bool FULL>
+__global__ void __launch_bounds__(quantize_threads(G)) k_quantize_rows(QuantizeParams P) {
+  constexpr int V = RowType<T>::V;
+  const int lane = threadIdx.x % G;
+  const int64_t row = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) / G;
+  const bool live = row < P.n;  // G = 32: whole warps; G > 32: one row a block, always live
+  if (!live) return;
+  const int d = P.d;
+
+  // where the row goes; of equal slots the last row's write stays
+  int64_t dst = row;
+  if (P.slots) {
+    dst = slot_at(P.slots, P.slot64, row);
+    bool mine = dst >= 0 && dst < P.capacity;
+    if (mine && P.claimed) {
+      mine = __ldcg(reinterpret_cast<const uint32_t*>(P.scales + dst)) == claim_tag(row);
+    } else if (mine) {
+      int later = 0;
+      for (int64_t j = row + 1 + lane; j < P.n; j += G) later |= slot_at(P.slots, P.slot64, j) == dst;
+      if constexpr (G > 32) later = __syncthreads_or(later);
+      else later = __any_sync(FULL_MASK, later);
+      mine = !later;
+    }
+    if constexpr (G > 32) {
+      if (P.claimed) mine = __syncthreads_and(mine);  // every thread has read the claim before it is overwritten
+    } else {
+      mine = __all_sync(FULL_MASK, mine);
+    }
+    if (!mine) dst = -1;
+    if (dst < 0 && !(FULL && P.res)) return;
+  }
+
+  const T* x = reinterpret_cast<const T*>(P.x) + row * P.x_stride;
+  Vec<T> v[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) v[k] = load_vec(x, (k * G + lane) * V, d, P.wide_in & 1);
+  if constexpr (FULL) {
+    if (P.res) {
+      const T* r = reinterpret_cast<const T*>(P.res) + row * P.res_stride;
+      T* s = reinterpret_cast<T*>(P.sum) + row * P.sum_stride;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const Vec<T> b = load_vec(r, (k * G + lane) * V, d, P.wide_in & 2);
+        // the sum is kept in the row's type, as the next layer reads it; the
+        // norm and the codes are those of the kept value
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[k].e[i] = RowType<T>::put(RowType<T>::get(v[k].e[i]) + RowType<T>::get(b.e[i]));
+        store_vec(s, (k * G + lane) * V, d, P.wide_in & 4, v[k]);
+      }
+    }
+  }
+
+  float wt[FULL ? NV : 1][FULL ? V : 1];
+  if constexpr (FULL) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * G + lane) * V;
+      if (!P.w) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) wt[k][i] = 1.f;
+      } else if (P.w_f32) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) wt[k][i] = c + i < d ? __ldg(reinterpret_cast<const float*>(P.w) + c + i) : 0.f;
+      } else {
+        const Vec<T> b = load_vec(reinterpret_cast<const T*>(P.w), c, d, P.wide_in & 8);
+#pragma unroll
+        for (int i = 0; i < V; ++i) wt[k][i] = RowType<T>::get(b.e[i]);
+      }
+    }
+  }
+
+  RowSums r{0.f, 0.f, 0.f, 0};
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float e = RowType<T>::get(v[k].e[i]);
+      float a = fabsf(e);
+      if constexpr (FULL) {
+        r.ss = fmaf(e, e, r.ss);
+        const float aw = fabsf(wt[k][i]), p = a * aw;
+        if (p >= r.top) raise(r.top, r.low, p, fmaf(a, aw, -p));  // fma gives the product's rounding error
+        a = p;
+      } else {
+        r.top = fmaxf(r.top, a);
+      }
+      r.bad |= !(a <= FLT_MAX);
+    }
+  r = reduce<G>(r);
+
+  float scale = r.top / 127.f;
+  if (FULL && P.norm && r.top > 0.f && !r.bad) {
+    if (r.ss > 1e-25f && r.ss < FLT_MAX) {
+      scale /= sqrtf(fmaf(r.ss, P.inv_n, P.eps));
+    } else {
+      // the squares left the range of 32 bits: sum them again as (v 2^-e)^2
+      RowSums m{0.f, 0.f, 0.f, 0};
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) m.top = fmaxf(m.top, fabsf(RowType<T>::get(v[k].e[i])));
+      m = reduce<G>(m);
+      const int e = ilogbf(m.top);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float s = ldexpf(RowType<T>::get(v[k].e[i]), -e);
+          m.ss = fmaf(s, s, m.ss);
+        }
+      m = reduce<G>(m);
+      const double mean = ldexp((double)m.ss * (double)P.inv_n, 2 * e) + (double)P.eps;
+      scale = (float)((double)r.top / 127.0 / sqrt(mean));
+    }
+  }
+  if (dst < 0) return;
+  if (r.bad) scale = __uint_as_float(0x7fffffffu);  // a NaN without the sign that marks claims
+  if (lane == 0) P.scales[dst] = scale;
+
+  // tiny rows are brought into range by a power of two, so 127 / a stays finite
+  const float pre = r.top < 1e-18f ? 1.2089258196146292e24f : 1.f;  // 2^80
+  const float inv = r.bad || r.top == 0.f ? 0.f : 127.f / (r.top * pre);
+  const double a = (double)r.top + (double)r.low;
+  int8_t* out = P.codes + dst * P.code_stride;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    union {
+      int8_t b[V];
+      uint32_t w[V / 4];
+    } q;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float e = RowType<T>::get(v[k].e[i]);
+      float w = 1.f;
+      if constexpr (FULL) w = wt[k][i];
+      const float t = e * w * pre * inv, n = rintf(t);
+      int code = (int)n;
+      if (fabsf(t - n) > NEAR_HALF) code = code_near_half(e, w, a);
+      q.b[i] = r.bad ? (int8_t)0 : (int8_t)code;
+    }
+    const int c = (k * G + lane) * V;
+    if (P.wide_out && c + V <= d) {
+      if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + c) = q.w[0];
+      else *reinterpret_cast<uint2*>(out + c) = make_uint2(q.w[0], q.w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c + i < d) out[c + i] = q.b[i];
+    }
+  }
+}
+
+// ---------------------------------------------------------------- rows read back
+struct ReadParams {
+  const int8_t* codes;
+  const float* scales;
+  const void* ids;  // nullptr: row i
+  void* out;
+  int64_t n, rows, code_stride, out_stride;
+  int d, id64, wide_in, wide_out;
+};
+
+// A warp a row: 16 bytes of output a lane and step.  An id below 0 is an empty
+// place (zeros), one past the store a mistake (NaN).
+template <typename T>
+__global__ void __launch_bounds__(256) k_dequantize_rows(ReadParams P) {
+  constexpr int V = RowType<T>::V;
+  const int lane = threadIdx.x & 31;
+  const int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
+  if (i >= P.n) return;
+  const int64_t id = P.ids ? slot_at(P.ids, P.id64, i) : i;
+  const bool known = id >= 0 && id < P.rows;
+  const float scale = known ? __ldg(P.scales + id) : id < 0 ? 0.f : __uint_as_float(0x7fffffffu);
+  const int8_t* in = P.codes + (known ? id : 0) * P.code_stride;
+  T* out = reinterpret_cast<T*>(P.out) + i * P.out_stride;
+  for (int c = lane * V; c < P.d; c += 32 * V) {
+    union {
+      int8_t b[V];
+      uint32_t w[V / 4];
+    } q;
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) q.w[k] = 0;
+    if (known) {
+      if (P.wide_in && c + V <= P.d) {
+        if constexpr (V == 4) {
+          q.w[0] = __ldg(reinterpret_cast<const uint32_t*>(in + c));
+        } else {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(in + c));
+          q.w[0] = w.x;
+          q.w[1] = w.y;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (c + k < P.d) q.b[k] = __ldg(in + c + k);
+      }
+    }
+    Vec<T> v;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v.e[k] = RowType<T>::put((float)q.b[k] * scale);  // the value's one rounding
+    store_vec(out, c, P.d, P.wide_out, v);
+  }
+}
+
+// ---------------------------------------------------------------- products
+struct ScoresParams {
+  const int8_t* q;
+  const float* q_scales;
+  const int8_t* codes;
+  const float* scales;
+  const float* bias;  // nullptr: none
+  void* out;
+  int64_t nq, n, q_stride, code_stride, out_stride;
+  int d;
+};
+
+template <typename T>
+__device__ __forceinline__ T scored(int acc, float sq, float sr, float bias) {
+  return RowType<T>::put(fmaf((float)acc * sq, sr, bias));
+}
+
+// Eight lanes a row, each with 16 codes a step, NQ queries in shared memory
+// (zero past d, so what a row's padding holds does not count).
+template <typename T, int NQ>
+__global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
+  extern __shared__ __align__(16) int8_t s_q[];
+  const int chunks = (P.d + 15) >> 4;
+  const int64_t q0 = (int64_t)blockIdx.y * NQ;
+  for (int i = threadIdx.x; i < NQ * chunks * 16; i += blockDim.x) {
+    const int q = i / (chunks * 16), c = i - q * (chunks * 16);
+    s_q[i] = q0 + q < P.nq && c < P.d ? P.q[(q0 + q) * P.q_stride + c] : (int8_t)0;
+  }
+  __syncthreads();
+  const int sub = threadIdx.x & 7;
+  const int64_t groups = (int64_t)gridDim.x * (blockDim.x >> 3);
+  // whole warps stay in the loop together: the shuffles need every lane
+  for (int64_t row0 = (blockIdx.x * (int64_t)blockDim.x + (threadIdx.x & ~31)) >> 3; row0 < P.n; row0 += groups) {
+    const int64_t row = row0 + ((threadIdx.x & 31) >> 3);
+    const bool live = row < P.n;
+    const int4* r = reinterpret_cast<const int4*>(P.codes + (live ? row : 0) * P.code_stride);
+    int acc[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) acc[q] = 0;
+    for (int c = sub; c < chunks; c += 8) {
+      const int4 b = __ldg(r + c);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int4 a = reinterpret_cast<const int4*>(s_q)[q * chunks + c];
+        acc[q] = __dp4a(a.x, b.x, __dp4a(a.y, b.y, __dp4a(a.z, b.z, __dp4a(a.w, b.w, acc[q]))));
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) acc[q] += __shfl_xor_sync(FULL_MASK, acc[q], o);
+      if (live && sub == (q & 7) && q0 + q < P.nq)
+        reinterpret_cast<T*>(P.out)[(q0 + q) * P.out_stride + row] =
+            scored<T>(acc[q], __ldg(P.q_scales + q0 + q), __ldg(P.scales + row), P.bias ? __ldg(P.bias + row) : 0.f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+static int bad(const char* msg) {
+  try {
+    cb::set_error(msg);
+  } catch (...) {
+  }
+  return CIRCUIT_ERR_ARG;
+}
+static int check(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return CIRCUIT_OK;
+  try {
+    cb::cuda_ok(e, what);
+  } catch (...) {
+  }
+  return CIRCUIT_ERR_CUDA;
+}
+static bool on16(const void* p, int64_t stride_bytes) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)stride_bytes) & 15) == 0;
+}
+static int type_bytes(int dtype) { return dtype == CIRCUIT_F32 ? 4 : dtype == CIRCUIT_F16 || dtype == CIRCUIT_BF16 ? 2 : 0; }
+
+template <typename T, int G, int NV, bool FULL>
+static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
+  constexpr int threads = quantize_threads(G);
+  const int64_t blocks = G == 32 ? (P.n + 7) / 8 : P.n;
+  k_quantize_rows<T, G, NV, FULL><<<(unsigned)blocks, threads, 0, st>>>(P);
+}
+template <typename T, int G, bool FULL>
+static void quantize_nv(const QuantizeParams& P, int vectors, cudaStream_t st) {
+  const int nv = (vectors + G - 1) / G;
+  if (nv <= 1) launch_quantize<T, G, 1, FULL>(P, st);
+  else if (nv <= 2) launch_quantize<T, G, 2, FULL>(P, st);
+  else if (nv <= 3) launch_quantize<T, G, 3, FULL>(P, st);
+  else if (G < 512 || RowType<T>::V == 8 || nv <= 4) launch_quantize<T, G, 4, FULL>(P, st);
+  else if constexpr (G == 512 && RowType<T>::V == 4) launch_quantize<T, G, 8, FULL>(P, st);
+}
+// Threads a row: a warp while it holds the row in at most 4 vectors a lane,
+// then a block of 128, then of 512 (up to 8 vectors for 16,384 fp32 values).
+template <typename T, bool FULL>
+static void quantize(const QuantizeParams& P, cudaStream_t st) {
+  const int vectors = (P.d + RowType<T>::V - 1) / RowType<T>::V;
+  if (vectors <= 32 * 4) quantize_nv<T, 32, FULL>(P, vectors, st);
+  else if (vectors <= 128 * 4) quantize_nv<T, 128, FULL>(P, vectors, st);
+  else quantize_nv<T, 512, FULL>(P, vectors, st);
+}
+
+template <typename T, int NQ>
+static int launch_rows(const ScoresParams& P, cudaStream_t st) {
+  const int smem = NQ * ((P.d + 15) / 16) * 16;
+  if (smem > 48 * 1024) {
+    const int rc = check(cudaFuncSetAttribute(k_scores_rows<T, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                         "int8_scores shared memory");
+    if (rc) return rc;
+  }
+  const int64_t blocks = (P.n + 31) / 32;
+  const dim3 grid((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), (unsigned)((P.nq + NQ - 1) / NQ));
+  k_scores_rows<T, NQ><<<grid, 256, smem, st>>>(P);
+  return CIRCUIT_OK;
+}
+template <typename T>
+static int scores(const ScoresParams& P, cudaStream_t st) {
+  if (P.nq <= 1) return launch_rows<T, 1>(P, st);
+  if (P.nq <= 2) return launch_rows<T, 2>(P, st);
+  if (P.nq <= 4) return launch_rows<T, 4>(P, st);
+  return launch_rows<T, 8>(P, st);
+}
+
+}  // namespace i8
+}  // namespace cb
+
+using namespace cb::i8;
+
+extern "C" {
+
+int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, int64_t row_stride,
+                             const void* residual, int64_t residual_stride, const void* weight, int weight_dtype,
+                             int norm, float eps, void* summed, int64_t summed_stride, const void* slots,
+                             int slot_bytes, int64_t capacity, int8_t* codes, int64_t code_stride, float* scales,
+                             void* stream) {
+  const int e = type_bytes(dtype);
+  if (!e) return bad("quantize_rows: dtype must be CIRCUIT_F32, CIRCUIT_F16 or CIRCUIT_BF16");
+  if (dim < 1 || dim > CIRCUIT_INT8_MAX_DIM) return bad("quantize_rows: dim must be in [1, 16384]");
+  if (n < 0 || n > 0x7fffffffLL) return bad("quantize_rows: n must be in [0, 2^31)");
+  if (norm < CIRCUIT_NORM_NONE || norm > CIRCUIT_NORM_UNIT) return bad("quantize_rows: unknown norm");
+  if (norm == CIRCUIT_NORM_NONE && (residual || weight))
+    return bad("quantize_rows: residual and weight need a norm");
+  if (!(eps >= 0.f && eps <= FLT_MAX)) return bad("quantize_rows: eps must be finite and not negative");
+  if (weight && weight_dtype != dtype && weight_dtype != CIRCUIT_F32)
+    return bad("quantize_rows: the weight must be of the rows' type or fp32");
+  if (slots && slot_bytes != 4 && slot_bytes != 8) return bad("quantize_rows: slots must be int32 or int64");
+  if (capacity < 0) return bad("quantize_rows: negative capacity");
+  if (n == 0) return CIRCUIT_OK;
+  if (!rows || !codes || !scales || (residual && !summed)) return bad("quantize_rows: null pointer");
+  if (!slots && capacity < n) return bad("quantize_rows: more rows than the output holds");
+  if (row_stride < dim || code_stride < dim || (residual && (residual_stride < dim || summed_stride < dim)))
+    return bad("quantize_rows: a row stride is smaller than dim");
+  const uintptr_t align = (uintptr_t)rows | (uintptr_t)residual | (residual ? (uintptr_t)summed : 0);
+  if (align % e || (weight && (uintptr_t)weight % (weight_dtype == CIRCUIT_F32 ? 4 : 2)) || (uintptr_t)scales % 4 ||
+      (slots && (uintptr_t)slots % slot_bytes))
+    return bad("quantize_rows: a pointer is not aligned to its type");
+  QuantizeParams P{};
+  P.x = rows;
+  P.res = residual;
+  P.w = weight;
+  P.sum = summed;
+  P.slots = slots;
+  P.codes = codes;
+  P.scales = scales;
+  P.n = n;
+  P.x_stride = row_stride;
+  P.res_stride = residual_stride;
+  P.sum_stride = summed_stride;
+  P.code_stride = code_stride;
+  P.capacity = capacity;
+  P.d = dim;
+  P.w_f32 = weight && weight_dtype == CIRCUIT_F32;
+  P.norm = norm;
+  P.inv_n = norm == CIRCUIT_NORM_RMS ? 1.f / (float)dim : 1.f;
+  P.eps = eps;
+  P.slot64 = slot_bytes == 8;
+  // one access a vector where the rows allow it
+  P.wide_in = (on16(rows, row_stride * e) ? 1 : 0) | (residual && on16(residual, residual_stride * e) ? 2 : 0) |
+              (residual && on16(summed, summed_stride * e) ? 4 : 0) | (weight && on16(weight, 0) ? 8 : 0);
+  P.wide_out = (((uintptr_t)codes | (uintptr_t)code_stride) & 7) == 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  // Equal slots: each row of a short write looks through the later ones; a long
+  // write claims its slots first, the claims standing in the scales.
+  P.claimed = slots && n > 1024;
+  if (P.claimed) {
+    const unsigned blocks = (unsigned)((n + 255) / 256);
+    k_reset_slots<<<blocks, 256, 0, st>>>(slots, P.slot64, n, capacity, scales);
+    k_claim_slots<<<blocks, 256, 0, st>>>(slots, P.slot64, n, capacity, scales);
+  }
+  const bool full = norm != CIRCUIT_NORM_NONE;
+  if (dtype == CIRCUIT_F32) full ? quantize<float, true>(P, st) : quantize<float, false>(P, st);
+  else if (dtype == CIRCUIT_F16) full ? quantize<__half, true>(P, st) : quantize<__half, false>(P, st);
+  else full ? quantize<__nv_bfloat16, true>(P, st) : quantize<__nv_bfloat16, false>(P, st);
+  return check(cudaGetLastError(), "quantize_rows launch");
+}
+
+int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const float* scales, int64_t rows, int dim,
+                               const void* ids, int id_bytes, int64_t n, void* out, int dtype, int64_t out_stride,
+                               void* stream) {
+  const int e = type_bytes(dtype);
+  if (!e) return bad("dequantize_rows: dtype must be CIRCUIT_F32, CIRCUIT_F16 or CIRCUIT_BF16");
+  if (dim < 1 || dim > CIRCUIT_INT8_MAX_DIM) return bad("dequantize_rows: dim must be in [1, 16384]");
+  if (n < 0 || n > 0x7fffffffLL || rows < 0) return bad("dequantize_rows: bad sizes");
+  if (ids && id_bytes != 4 && id_bytes != 8) return bad("dequantize_rows: ids must be int32 or int64");
+  if (n == 0) return CIRCUIT_OK;
+  if (!codes || !scales || !out) return bad("dequantize_rows: null pointer");
+  if (!ids && rows < n) return bad("dequantize_rows: more rows asked for than there are");
+  if (code_stride < dim || out_stride < dim) return bad("dequantize_rows: a row stride is smaller than dim");
+  if ((uintptr_t)out % e || (uintptr_t)scales % 4 || (ids && (uintptr_t)ids % id_bytes))
+    return bad("dequantize_rows: a pointer is not aligned to its type");
+  ReadParams P{codes, scales, ids, out, n, rows, code_stride, out_stride, dim, id_bytes == 8,
+               (((uintptr_t)codes | (uintptr_t)code_stride) & 7) == 0, on16(out, out_stride * e)};
+  cudaStream_t st = (cudaStream_t)stream;
+  const unsigned blocks = (unsigned)((n + 7) / 8);
+  if (dtype == CIRCUIT_F32) k_dequantize_rows<float><<<blocks, 256, 0, st>>>(P);
+  else if (dtype == CIRCUIT_F16) k_dequantize_rows<__half><<<blocks, 256, 0, st>>>(P);
+  else k_dequantize_rows<__nv_bfloat16><<<blocks, 256, 0, st>>>(P);
+  return check(cudaGetLastError(), "dequantize_rows launch");
+}
+
+int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const float* query_scales, int64_t num_queries,
+                           const int8_t* codes, int64_t code_stride, const float* scales, int64_t n, int dim,
+                           const float* bias, void* out, int dtype, int64_t out_stride, void* stream) {
+  const int e = type_bytes(dtype);
+  if (!e) return bad("int8_scores: dtype must be CIRCUIT_F32, CIRCUIT_F16 or CIRCUIT_BF16");
+  if (dim < 1 || dim > CIRCUIT_INT8_MAX_DIM) return bad("int8_scores: dim must be in [1, 16384]");
+  if (num_queries < 0 || num_queries > CIRCUIT_INT8_MAX_QUERIES)
+    return bad("int8_scores: the number of queries must be in [0, 65535]");
+  if (n < 0 || n > 0x7fffffffLL) return bad("int8_scores: n must be in [0, 2^31)");
+  if (num_queries == 0 || n == 0) return CIRCUIT_OK;
+  if (!queries || !query_scales || !codes || !scales || !out) return bad("int8_scores: null pointer");
+  const int64_t padded = (dim + 15) / 16 * 16;
+  if (query_stride < padded || code_stride < padded || !on16(queries, query_stride) || !on16(codes, code_stride))
+    return bad("int8_scores: code rows must start on 16 bytes and be padded to a multiple of 16");
+  if (out_stride < n) return bad("int8_scores: out_stride is smaller than n");
+  if ((uintptr_t)out % e || ((uintptr_t)query_scales | (uintptr_t)scales | (uintptr_t)bias) % 4)
+    return bad("int8_scores: a pointer is not aligned to its type");
+  const ScoresParams P{queries, query_scales, codes, scales, bias, out, num_queries, n, query_stride, code_stride,
+                       out_stride, dim};
+  cudaStream_t st = (cudaStream_t)stream;
+  const int rc = dtype == CIRCUIT_F32   ? scores<float>(P, st)
+                 : dtype == CIRCUIT_F16 ? scores<__half>(P, st)
+                                        : scores<__nv_bfloat16>(P, st);
+  return rc ? rc : check(cudaGetLastError(), "int8_scores launch");
+}
+
+}  // extern "C"

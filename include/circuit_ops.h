@@ -86,6 +86,49 @@ int circuit_op_hierarchical_search(const float* query, const float* root_centers
                                    int num_total_children, int64_t n, int dim, float threshold, int rank,
                                    float query_norm, void* stream);
 
+/* ---------------------------------------------------------------- rows in 8 bits
+ * A row of dim values is kept as dim int8 codes and one fp32 scale; code c stands for c * scale.  These ops run on the
+ * device of their pointers, which must be the current one, allocate nothing, and may be captured into a CUDA graph.
+ * Strides are in elements of the tensor they belong to (codes: bytes); dim is at most CIRCUIT_INT8_MAX_DIM. */
+#define CIRCUIT_INT8_MAX_DIM 16384
+#define CIRCUIT_INT8_MAX_QUERIES 65535
+
+/* value types */
+#define CIRCUIT_F32 0
+#define CIRCUIT_F16 1
+#define CIRCUIT_BF16 2
+
+/* norms of circuit_op_quantize_rows */
+#define CIRCUIT_NORM_NONE 0 /* scale = max|x| / 127 */
+#define CIRCUIT_NORM_RMS 1  /* divided by sqrt(mean(v^2) + eps) */
+#define CIRCUIT_NORM_UNIT 2 /* divided by sqrt(sum(v^2) + eps) */
+
+/* Quantises n rows: v = rows (+ residual, rounded once to the rows' type and written to `summed`), u = v * weight,
+ * codes = rint(127 u / max|u|) of the real quotient (ties to even), scale = max|u| / 127 over the norm.
+ * residual and weight (of the rows' type or fp32, dim values) may be NULL; both need a norm.  A row of zeros gets scale
+ * 0; a row with an infinity, a NaN, or a product beyond fp32 gets codes 0 and scale NaN.
+ * slots == NULL: row i is written to row i of codes / scales.  Otherwise to row slots[i] (int32 or int64 as slot_bytes
+ * says) of the `capacity` rows: a slot outside [0, capacity) writes nothing, of equal slots the last row stays, other
+ * rows are left as they are.  `summed` may be `rows` or `residual` itself. */
+int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, int64_t row_stride,
+                             const void* residual, int64_t residual_stride, const void* weight, int weight_dtype,
+                             int norm, float eps, void* summed, int64_t summed_stride, const void* slots,
+                             int slot_bytes, int64_t capacity, int8_t* codes, int64_t code_stride, float* scales,
+                             void* stream);
+
+/* out[i] = codes[id] * scales[id] for id = ids[i] (int32 or int64), or i when ids == NULL, rounded once to dtype.
+ * A negative id is an empty place and gives zeros, an id >= rows gives NaN. */
+int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const float* scales, int64_t rows, int dim,
+                               const void* ids, int id_bytes, int64_t n, void* out, int dtype, int64_t out_stride,
+                               void* stream);
+
+/* out[i][j] = query_scales[i] * scales[j] * sum_k queries[i][k] codes[j][k] (+ bias[j]), rounded once to dtype; the
+ * sum is exact (32-bit integers).  Code rows start on 16 bytes and their strides are multiples of 16; up to 15 bytes
+ * past dim are read in each row (the last one's too) and do not count. */
+int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const float* query_scales, int64_t num_queries,
+                           const int8_t* codes, int64_t code_stride, const float* scales, int64_t n, int dim,
+                           const float* bias, void* out, int dtype, int64_t out_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
