@@ -45,6 +45,7 @@ EXPORTED_SYMBOLS = (
     "circuit_op_quantize_rows",
     "circuit_op_dequantize_rows",
     "circuit_op_int8_scores",
+    "circuit_op_int8_status",
     "circuit_merge_topk",
     "circuit_merge_topk_batch",
     "circuit_plan_shards",
@@ -127,6 +128,7 @@ def _declare(lib):
                                           _I64, _P, _P]),
         "circuit_op_dequantize_rows": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I64, _P, _I, _I64, _P]),
         "circuit_op_int8_scores": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _P, _P, _I, _I64, _P]),
+        "circuit_op_int8_status": (_I, [_P]),
         "circuit_merge_topk": (_I, [_P, _P, _I, _I, _P, _P, _P]),
         "circuit_merge_topk_batch": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
         "circuit_plan_shards": (_I, [_P, _I, _I, _P, _P]),

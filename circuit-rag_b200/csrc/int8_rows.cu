@@ -1,7 +1,7 @@
 // Rows in 8 bits (include/circuit_ops.h, the int8 section): quantisation with
 // one scale a row (plain, after a root-mean-square norm with the residual's
 // addition, or to unit length; into consecutive rows or into the slots of a row
-// store), reading rows back by id, and products of 8-bit queries with 8-bit rows.
+// store), and reading rows back by id.
 //
 // Mathematics.  With v = x (+ residual, rounded once to the row's type) and
 // u = v * w, a row's codes are rint(127 u_j / a), a = max|u|, and its scale is
@@ -10,74 +10,11 @@
 // gives the correctly rounded code of the real quotient (see code_of), and only
 // the scale carries the rounding of the 32-bit sum of squares.
 #include <cfloat>
-#include <cstdint>
-#include <string>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "../../include/circuit_ops.h"
-#include "common.cuh"
-#include "index_internal.h"
+#include "int8.cuh"
 
 namespace cb {
 namespace i8 {
-
-// ---------------------------------------------------------------- row types
-template <typename T>
-struct RowType;  // V: elements of a 16-byte vector
-template <>
-struct RowType<float> {
-  static constexpr int V = 4;
-  __device__ static float get(float x) { return x; }
-  __device__ static float put(float x) { return x; }
-};
-template <>
-struct RowType<__half> {
-  static constexpr int V = 8;
-  __device__ static float get(__half x) { return __half2float(x); }
-  __device__ static __half put(float x) { return __float2half_rn(x); }
-};
-template <>
-struct RowType<__nv_bfloat16> {
-  static constexpr int V = 8;
-  __device__ static float get(__nv_bfloat16 x) { return __bfloat162float(x); }
-  __device__ static __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
-};
-
-template <typename T>
-union Vec {
-  uint4 raw;
-  T e[RowType<T>::V];
-};
-
-// Elements [c, c + V) of a row of d elements: one 16-byte access where the row
-// allows it, else one access an element; zeros past the row's end.
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* row, int c, int d, bool wide) {
-  constexpr int V = RowType<T>::V;
-  Vec<T> v;
-  v.raw = make_uint4(0, 0, 0, 0);
-  if (wide && c + V <= d) {
-    v.raw = *reinterpret_cast<const uint4*>(row + c);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (c + i < d) v.e[i] = row[c + i];
-  }
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ void store_vec(T* row, int c, int d, bool wide, const Vec<T>& v) {
-  constexpr int V = RowType<T>::V;
-  if (wide && c + V <= d) {
-    *reinterpret_cast<uint4*>(row + c) = v.raw;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (c + i < d) row[c + i] = v.e[i];
-  }
-}
 
 // ---------------------------------------------------------------- reductions over the G threads of a row
 struct RowSums {
@@ -375,85 +312,7 @@ __global__ void __launch_bounds__(256) k_dequantize_rows(ReadParams P) {
   }
 }
 
-// ---------------------------------------------------------------- products
-struct ScoresParams {
-  const int8_t* q;
-  const float* q_scales;
-  const int8_t* codes;
-  const float* scales;
-  const float* bias;  // nullptr: none
-  void* out;
-  int64_t nq, n, q_stride, code_stride, out_stride;
-  int d;
-};
-
-template <typename T>
-__device__ __forceinline__ T scored(int acc, float sq, float sr, float bias) {
-  return RowType<T>::put(fmaf((float)acc * sq, sr, bias));
-}
-
-// Eight lanes a row, each with 16 codes a step, NQ queries in shared memory
-// (zero past d, so what a row's padding holds does not count).
-template <typename T, int NQ>
-__global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
-  extern __shared__ __align__(16) int8_t s_q[];
-  const int chunks = (P.d + 15) >> 4;
-  const int64_t q0 = (int64_t)blockIdx.y * NQ;
-  for (int i = threadIdx.x; i < NQ * chunks * 16; i += blockDim.x) {
-    const int q = i / (chunks * 16), c = i - q * (chunks * 16);
-    s_q[i] = q0 + q < P.nq && c < P.d ? P.q[(q0 + q) * P.q_stride + c] : (int8_t)0;
-  }
-  __syncthreads();
-  const int sub = threadIdx.x & 7;
-  const int64_t groups = (int64_t)gridDim.x * (blockDim.x >> 3);
-  // whole warps stay in the loop together: the shuffles need every lane
-  for (int64_t row0 = (blockIdx.x * (int64_t)blockDim.x + (threadIdx.x & ~31)) >> 3; row0 < P.n; row0 += groups) {
-    const int64_t row = row0 + ((threadIdx.x & 31) >> 3);
-    const bool live = row < P.n;
-    const int4* r = reinterpret_cast<const int4*>(P.codes + (live ? row : 0) * P.code_stride);
-    int acc[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) acc[q] = 0;
-    for (int c = sub; c < chunks; c += 8) {
-      const int4 b = __ldg(r + c);
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const int4 a = reinterpret_cast<const int4*>(s_q)[q * chunks + c];
-        acc[q] = __dp4a(a.x, b.x, __dp4a(a.y, b.y, __dp4a(a.z, b.z, __dp4a(a.w, b.w, acc[q]))));
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) acc[q] += __shfl_xor_sync(FULL_MASK, acc[q], o);
-      if (live && sub == (q & 7) && q0 + q < P.nq)
-        reinterpret_cast<T*>(P.out)[(q0 + q) * P.out_stride + row] =
-            scored<T>(acc[q], __ldg(P.q_scales + q0 + q), __ldg(P.scales + row), P.bias ? __ldg(P.bias + row) : 0.f);
-    }
-  }
-}
-
 // ---------------------------------------------------------------- host side
-static int bad(const char* msg) {
-  try {
-    cb::set_error(msg);
-  } catch (...) {
-  }
-  return CIRCUIT_ERR_ARG;
-}
-static int check(cudaError_t e, const char* what) {
-  if (e == cudaSuccess) return CIRCUIT_OK;
-  try {
-    cb::cuda_ok(e, what);
-  } catch (...) {
-  }
-  return CIRCUIT_ERR_CUDA;
-}
-static bool on16(const void* p, int64_t stride_bytes) {
-  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)stride_bytes) & 15) == 0;
-}
-static int type_bytes(int dtype) { return dtype == CIRCUIT_F32 ? 4 : dtype == CIRCUIT_F16 || dtype == CIRCUIT_BF16 ? 2 : 0; }
-
 template <typename T, int G, int NV, bool FULL>
 static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
   constexpr int threads = quantize_threads(G);
@@ -477,27 +336,6 @@ static void quantize(const QuantizeParams& P, cudaStream_t st) {
   if (vectors <= 32 * 4) quantize_nv<T, 32, FULL>(P, vectors, st);
   else if (vectors <= 128 * 4) quantize_nv<T, 128, FULL>(P, vectors, st);
   else quantize_nv<T, 512, FULL>(P, vectors, st);
-}
-
-template <typename T, int NQ>
-static int launch_rows(const ScoresParams& P, cudaStream_t st) {
-  const int smem = NQ * ((P.d + 15) / 16) * 16;
-  if (smem > 48 * 1024) {
-    const int rc = check(cudaFuncSetAttribute(k_scores_rows<T, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                         "int8_scores shared memory");
-    if (rc) return rc;
-  }
-  const int64_t blocks = (P.n + 31) / 32;
-  const dim3 grid((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), (unsigned)((P.nq + NQ - 1) / NQ));
-  k_scores_rows<T, NQ><<<grid, 256, smem, st>>>(P);
-  return CIRCUIT_OK;
-}
-template <typename T>
-static int scores(const ScoresParams& P, cudaStream_t st) {
-  if (P.nq <= 1) return launch_rows<T, 1>(P, st);
-  if (P.nq <= 2) return launch_rows<T, 2>(P, st);
-  if (P.nq <= 4) return launch_rows<T, 4>(P, st);
-  return launch_rows<T, 8>(P, st);
 }
 
 }  // namespace i8
@@ -595,32 +433,6 @@ int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const f
   else if (dtype == CIRCUIT_F16) k_dequantize_rows<__half><<<blocks, 256, 0, st>>>(P);
   else k_dequantize_rows<__nv_bfloat16><<<blocks, 256, 0, st>>>(P);
   return check(cudaGetLastError(), "dequantize_rows launch");
-}
-
-int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const float* query_scales, int64_t num_queries,
-                           const int8_t* codes, int64_t code_stride, const float* scales, int64_t n, int dim,
-                           const float* bias, void* out, int dtype, int64_t out_stride, void* stream) {
-  const int e = type_bytes(dtype);
-  if (!e) return bad("int8_scores: dtype must be CIRCUIT_F32, CIRCUIT_F16 or CIRCUIT_BF16");
-  if (dim < 1 || dim > CIRCUIT_INT8_MAX_DIM) return bad("int8_scores: dim must be in [1, 16384]");
-  if (num_queries < 0 || num_queries > CIRCUIT_INT8_MAX_QUERIES)
-    return bad("int8_scores: the number of queries must be in [0, 65535]");
-  if (n < 0 || n > 0x7fffffffLL) return bad("int8_scores: n must be in [0, 2^31)");
-  if (num_queries == 0 || n == 0) return CIRCUIT_OK;
-  if (!queries || !query_scales || !codes || !scales || !out) return bad("int8_scores: null pointer");
-  const int64_t padded = (dim + 15) / 16 * 16;
-  if (query_stride < padded || code_stride < padded || !on16(queries, query_stride) || !on16(codes, code_stride))
-    return bad("int8_scores: code rows must start on 16 bytes and be padded to a multiple of 16");
-  if (out_stride < n) return bad("int8_scores: out_stride is smaller than n");
-  if ((uintptr_t)out % e || ((uintptr_t)query_scales | (uintptr_t)scales | (uintptr_t)bias) % 4)
-    return bad("int8_scores: a pointer is not aligned to its type");
-  const ScoresParams P{queries, query_scales, codes, scales, bias, out, num_queries, n, query_stride, code_stride,
-                       out_stride, dim};
-  cudaStream_t st = (cudaStream_t)stream;
-  const int rc = dtype == CIRCUIT_F32   ? scores<float>(P, st)
-                 : dtype == CIRCUIT_F16 ? scores<__half>(P, st)
-                                        : scores<__nv_bfloat16>(P, st);
-  return rc ? rc : check(cudaGetLastError(), "int8_scores launch");
 }
 
 }  // extern "C"

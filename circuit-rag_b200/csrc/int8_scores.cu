@@ -1,0 +1,341 @@
+// Products of 8-bit queries with 8-bit rows (circuit_op_int8_scores):
+// out[i][j] = sq_i sr_j sum_k q_ik c_jk + bias_j, the sum exact in 32-bit integers.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "int8.cuh"
+#include "tcgen05.cuh"
+
+namespace cb {
+namespace i8 {
+
+struct ScoresParams {
+  const int8_t* q;
+  const float* q_scales;
+  const int8_t* codes;
+  const float* scales;
+  const float* bias;  // nullptr: none
+  void* out;
+  int64_t nq, n, q_stride, code_stride, out_stride;
+  int d;
+};
+
+template <typename T>
+__device__ __forceinline__ T scored(int acc, float sq, float sr, float bias) {
+  return RowType<T>::put(fmaf((float)acc * sq, sr, bias));
+}
+
+// Eight lanes a row, each with 16 codes a step, NQ queries in shared memory
+// (zero past d, so what a row's padding holds does not count).
+template <typename T, int NQ>
+__global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
+  extern __shared__ __align__(16) int8_t s_q[];
+  const int chunks = (P.d + 15) >> 4;
+  const int64_t q0 = (int64_t)blockIdx.y * NQ;
+  for (int i = threadIdx.x; i < NQ * chunks * 16; i += blockDim.x) {
+    const int q = i / (chunks * 16), c = i - q * (chunks * 16);
+    s_q[i] = q0 + q < P.nq && c < P.d ? P.q[(q0 + q) * P.q_stride + c] : (int8_t)0;
+  }
+  __syncthreads();
+  const int sub = threadIdx.x & 7;
+  const int64_t groups = (int64_t)gridDim.x * (blockDim.x >> 3);
+  // whole warps stay in the loop together: the shuffles need every lane
+  for (int64_t row0 = (blockIdx.x * (int64_t)blockDim.x + (threadIdx.x & ~31)) >> 3; row0 < P.n; row0 += groups) {
+    const int64_t row = row0 + ((threadIdx.x & 31) >> 3);
+    const bool live = row < P.n;
+    const int4* r = reinterpret_cast<const int4*>(P.codes + (live ? row : 0) * P.code_stride);
+    int acc[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) acc[q] = 0;
+    for (int c = sub; c < chunks; c += 8) {
+      const int4 b = __ldg(r + c);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int4 a = reinterpret_cast<const int4*>(s_q)[q * chunks + c];
+        acc[q] = __dp4a(a.x, b.x, __dp4a(a.y, b.y, __dp4a(a.z, b.z, __dp4a(a.w, b.w, acc[q]))));
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) acc[q] += __shfl_xor_sync(FULL_MASK, acc[q], o);
+      if (live && sub == (q & 7) && q0 + q < P.nq)
+        reinterpret_cast<T*>(P.out)[(q0 + q) * P.out_stride + row] =
+            scored<T>(acc[q], __ldg(P.q_scales + q0 + q), __ldg(P.scales + row), P.bias ? __ldg(P.bias + row) : 0.f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- tensor-core products
+// One persistent CTA an SM.  A unit is 128 rows (the MMA's M) against BN queries
+// (its N); units are dealt round robin with the query tiles fastest, so a row
+// tile comes from HBM once and its other query tiles read it from L2.  A TMA warp
+// streams 128-byte K chunks of both operands through a 192 KB ring, one elected
+// thread issues the MMAs into one of two TMEM accumulators, and eight epilogue
+// warps scale the other one.  With rows as M, a lane of the accumulator is a row
+// and a column a query: each warp store writes 32 consecutive results of one
+// query's row of `out`, without a transposition.
+constexpr int MMA_ROWS = 128;
+constexpr int MMA_THREADS = 320;  // warps 0-7 epilogue, 8 TMA, 9 MMA
+constexpr int RING_BYTES = 192 * 1024;
+constexpr int chunk_bytes(int BN) { return (MMA_ROWS + BN) * 128; }
+constexpr int ring_stages(int BN) { return RING_BYTES / chunk_bytes(BN); }
+
+// Bits of the waits that gave up, kept until circuit_op_int8_status reads them.
+__device__ int g_error;
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(MMA_THREADS, 1)
+    k_scores_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
+                 int q_tiles, int64_t units) {
+  constexpr int S = ring_stages(BN), STAGE = chunk_bytes(BN), HALF = BN / 2;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ int s_failed;
+  __shared__ float s_sq[8][HALF];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = (P.d + 127) >> 7;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 8);  // one lane of each epilogue warp
+    }
+    s_failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) tc::tmem_alloc(&tmem_base, 2 * BN);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_base;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      int s = 0;
+      int64_t filled = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const int64_t rt = u / q_tiles;
+        const int row0 = (int)(rt * MMA_ROWS), q0 = (int)(u - rt * q_tiles) * BN;
+        for (int j = 0; j < chunks; ++j, ++filled) {
+          if (filled >= S && !mbar_wait(&empty[s], ph ^ 1u, &g_error, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
+          mbar_arrive_expect_tx(&full[s], STAGE);  // out-of-range rows and columns arrive as zeros
+          unsigned char* dst = smem + s * STAGE;
+          tc::tma_load_2d(dst, &cmap, 128 * j, row0, &full[s]);
+          tc::tma_load_2d(dst + MMA_ROWS * 128, &qmap, 128 * j, q0, &full[s]);
+          if (++s == S) { s = 0; ph ^= 1u; }
+        }
+      }
+      // the last commits to the empty barriers have landed before this CTA exits
+      for (int64_t t = filled > S ? filled - S : 0; t < filled && ok; ++t)
+        ok = mbar_wait(&empty[t % S], (uint32_t)(t / S) & 1u, &g_error, ERR_TIMEOUT_EMPTY);
+      if (!ok) s_failed = 1;
+    }
+  } else if (warp == 9) {
+    constexpr uint32_t idesc = tc::idesc_s8(MMA_ROWS, BN);
+    const uint32_t sbase = smem_u32(smem);
+    const uint64_t dA = tc::sdesc_k_sw128(sbase), dB = tc::sdesc_k_sw128(sbase + MMA_ROWS * 128);
+    const int tail = (P.d - (chunks - 1) * 128 + 31) >> 5;  // K steps of 32 in the last chunk
+    int s = 0, it = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++it) {
+      const int b = it & 1;
+      if (it >= 2 && !__all_sync(FULL_MASK, mbar_wait(&acc_empty[b], (uint32_t)(it / 2 - 1) & 1u, &g_error,
+                                                      ERR_TIMEOUT_EMPTY))) {
+        ok = false;
+        break;
+      }
+      tc::fence_after();
+      const uint32_t acc = tmem + (uint32_t)(b * BN);
+      for (int j = 0; j < chunks; ++j) {
+        if (!__all_sync(FULL_MASK, mbar_wait(&full[s], ph, &g_error, ERR_TIMEOUT_FULL))) { ok = false; break; }
+        tc::fence_after();
+        if (tc::elect_one()) {
+          const uint64_t off = (uint64_t)((uint32_t)(s * STAGE) >> 4);
+          const int steps = j + 1 < chunks ? 4 : tail;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 32 bytes of K further: 2 units of 16 bytes
+            if (k < steps) tc::mma_s8_ss(acc, dA + off + 2 * k, dB + off + 2 * k, idesc, (j | k) != 0 ? 1u : 0u);
+          tc::commit(&empty[s]);
+        }
+        __syncwarp();
+        if (++s == S) { s = 0; ph ^= 1u; }
+      }
+      if (ok && tc::elect_one()) tc::commit(&acc_full[b]);
+      __syncwarp();
+    }
+    if (!ok && lane == 0) s_failed = 1;
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
+    float* sq = s_sq[warp];
+    int64_t loaded = -1;
+    int it = 0;
+    bool ok = true;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x, ++it) {
+      const int b = it & 1;
+      const int64_t rt = u / q_tiles, row = rt * MMA_ROWS + 32 * quarter + lane;
+      const int64_t q0 = (u - rt * q_tiles) * BN + half * HALF;
+      const bool live = row < P.n;
+      const float sr = live ? __ldg(P.scales + row) : 0.f;
+      const float bias = live && P.bias ? __ldg(P.bias + row) : 0.f;
+      if (q0 != loaded) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < HALF; i += 32) sq[i + lane] = q0 + i + lane < P.nq ? __ldg(P.q_scales + q0 + i + lane) : 0.f;
+        __syncwarp();
+        loaded = q0;
+      }
+      // once a wait has given up, the results that it would have brought are NaN
+      ok = ok && __all_sync(FULL_MASK, mbar_wait(&acc_full[b], (uint32_t)(it / 2) & 1u, &g_error, ERR_TIMEOUT_FULL));
+      tc::fence_after();
+      T* out = reinterpret_cast<T*>(P.out) + q0 * P.out_stride + row;
+#pragma unroll 1
+      for (int c = 0; c < HALF; c += 32) {
+        uint32_t v[32];
+        tc::ld_32x32b_x32(tmem + lane_base + (uint32_t)(b * BN + half * HALF + c), v);
+        tc::wait_ld();
+        if (c + 32 == HALF) {
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[b]);
+        }
+        const int64_t left = P.nq - q0 - c;
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < left)
+              out[(c + i) * P.out_stride] =
+                  ok ? scored<T>((int)v[i], sq[c + i], sr, bias) : RowType<T>::put(__uint_as_float(0x7fffffffu));
+        }
+      }
+    }
+    if (!ok && lane == 0) s_failed = 1;
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (s_failed) grace_period();  // copies and MMAs of the failed waits end before the memory is freed
+  if (warp == 9) tc::tmem_dealloc(tmem, 2 * BN);
+}
+
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ok ? p : nullptr);
+  }();
+  return fn;
+}
+// [rows, d] codes as boxes of box_rows rows x 128 bytes, 128-byte swizzle.
+static bool code_map(CUtensorMap* map, const int8_t* base, int64_t rows, int d, int64_t stride, int box_rows) {
+  const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)stride};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+static int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
+
+template <typename T, int BN>
+static int launch_mma(const ScoresParams& P, cudaStream_t st) {
+  CUtensorMap qmap, cmap;
+  if (!code_map(&qmap, P.q, P.nq, P.d, P.q_stride, BN) || !code_map(&cmap, P.codes, P.n, P.d, P.code_stride, MMA_ROWS))
+    return bad("int8_scores: cuTensorMapEncodeTiled refused the code rows");
+  constexpr int smem = ring_stages(BN) * chunk_bytes(BN) + 1024;
+  const int rc = check(cudaFuncSetAttribute(k_scores_mma<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                       "int8_scores shared memory");
+  if (rc) return rc;
+  const int q_tiles = (int)((P.nq + BN - 1) / BN);
+  const int64_t units = (P.n + MMA_ROWS - 1) / MMA_ROWS * q_tiles, sms = sm_count();
+  k_scores_mma<T, BN><<<(unsigned)(units < sms ? units : sms), MMA_THREADS, smem, st>>>(qmap, cmap, P, q_tiles, units);
+  return CIRCUIT_OK;
+}
+
+template <typename T, int NQ>
+static int launch_rows(const ScoresParams& P, cudaStream_t st) {
+  const int smem = NQ * ((P.d + 15) / 16) * 16;
+  if (smem > 48 * 1024) {
+    const int rc = check(cudaFuncSetAttribute(k_scores_rows<T, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                         "int8_scores shared memory");
+    if (rc) return rc;
+  }
+  const int64_t blocks = (P.n + 31) / 32;
+  const dim3 grid((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), (unsigned)((P.nq + NQ - 1) / NQ));
+  k_scores_rows<T, NQ><<<grid, 256, smem, st>>>(P);
+  return CIRCUIT_OK;
+}
+template <typename T>
+static int scores(const ScoresParams& P, cudaStream_t st) {
+  if (P.nq <= 1) return launch_rows<T, 1>(P, st);
+  if (P.nq <= 2) return launch_rows<T, 2>(P, st);
+  if (P.nq <= 4) return launch_rows<T, 4>(P, st);
+  if (P.nq <= 8) return launch_rows<T, 8>(P, st);
+  if (P.nq <= 64) return launch_mma<T, 64>(P, st);
+  if (P.nq <= 128) return launch_mma<T, 128>(P, st);
+  return launch_mma<T, 256>(P, st);
+}
+
+}  // namespace i8
+}  // namespace cb
+
+using namespace cb::i8;
+
+extern "C" {
+
+int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const float* query_scales, int64_t num_queries,
+                           const int8_t* codes, int64_t code_stride, const float* scales, int64_t n, int dim,
+                           const float* bias, void* out, int dtype, int64_t out_stride, void* stream) {
+  const int e = type_bytes(dtype);
+  if (!e) return bad("int8_scores: dtype must be CIRCUIT_F32, CIRCUIT_F16 or CIRCUIT_BF16");
+  if (dim < 1 || dim > CIRCUIT_INT8_MAX_DIM) return bad("int8_scores: dim must be in [1, 16384]");
+  if (num_queries < 0 || num_queries > CIRCUIT_INT8_MAX_QUERIES)
+    return bad("int8_scores: the number of queries must be in [0, 65535]");
+  if (n < 0 || n > 0x7fffffffLL) return bad("int8_scores: n must be in [0, 2^31)");
+  if (num_queries == 0 || n == 0) return CIRCUIT_OK;
+  if (!queries || !query_scales || !codes || !scales || !out) return bad("int8_scores: null pointer");
+  const int64_t padded = (dim + 15) / 16 * 16;
+  if (query_stride < padded || code_stride < padded || !on16(queries, query_stride) || !on16(codes, code_stride))
+    return bad("int8_scores: code rows must start on 16 bytes and be padded to a multiple of 16");
+  if (out_stride < n) return bad("int8_scores: out_stride is smaller than n");
+  if ((uintptr_t)out % e || ((uintptr_t)query_scales | (uintptr_t)scales | (uintptr_t)bias) % 4)
+    return bad("int8_scores: a pointer is not aligned to its type");
+  const ScoresParams P{queries, query_scales, codes, scales, bias, out, num_queries, n, query_stride, code_stride,
+                       out_stride, dim};
+  cudaStream_t st = (cudaStream_t)stream;
+  const int rc = dtype == CIRCUIT_F32   ? scores<float>(P, st)
+                 : dtype == CIRCUIT_F16 ? scores<__half>(P, st)
+                                        : scores<__nv_bfloat16>(P, st);
+  return rc ? rc : check(cudaGetLastError(), "int8_scores launch");
+}
+
+int circuit_op_int8_status(void* stream) {
+  int rc = check(cudaStreamSynchronize((cudaStream_t)stream), "int8_status"), bits = 0;
+  const int none = 0;
+  if (!rc) rc = check(cudaMemcpyFromSymbol(&bits, g_error, sizeof(int)), "int8_status");
+  if (!rc && bits) rc = check(cudaMemcpyToSymbol(g_error, &none, sizeof(int)), "int8_status");
+  if (rc || !bits) return rc;
+  bad("int8_scores: a bounded wait on the device gave up; its results are NaN");
+  return CIRCUIT_ERR_TIMEOUT;
+}
+
+}  // extern "C"

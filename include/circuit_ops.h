@@ -129,6 +129,10 @@ int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const fl
                            const int8_t* codes, int64_t code_stride, const float* scales, int64_t n, int dim,
                            const float* bias, void* out, int dtype, int64_t out_stride, void* stream);
 
+/* Waits for `stream` and returns CIRCUIT_ERR_TIMEOUT if a bounded wait of circuit_op_int8_scores has given up on the
+ * current device since the last call (the results that it would have brought were written as NaN), else 0. */
+int circuit_op_int8_status(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from circuit_rag import _native
 from circuit_rag.int8 import dequantize_rows, int8_scores, quantize_rows, rms_norm_quantize
 
 pytestmark = pytest.mark.gpu
@@ -448,3 +449,7 @@ def test_together_on_a_side_stream_and_in_a_graph(nq):
         graph.replay()
         torch.cuda.synchronize()
         check(got)
+
+
+def test_no_wait_has_given_up():
+    assert _native.lib().circuit_op_int8_status(None) == 0
