@@ -17,11 +17,12 @@ from circuit_rag import _native
 
 _TYPES = {torch.float32: _native.CIRCUIT_F32, torch.float16: _native.CIRCUIT_F16,
           torch.bfloat16: _native.CIRCUIT_BF16}
+_MAX_DIM = _native.CIRCUIT_INT8_MAX_DIM
 
-
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
+# A small call is a few microseconds of host time: the current device and its stream are asked for as plain integers
+# (torch.cuda.current_stream() builds an object, 3.4 us), and messages are only formatted once a check has failed.
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _cuda(t, name: str) -> None:
@@ -29,122 +30,125 @@ def _cuda(t, name: str) -> None:
         raise RuntimeError(f"{name} must be CUDA tensor")
 
 
-def _rows(t: torch.Tensor, name: str, dtype=None) -> torch.Tensor:
-    """A [n, dim] tensor whose values lie next to each other in each row (a copy if they do not)."""
-    _cuda(t, name)
-    _need(t.ndim == 2, f"{name} must have shape [n, dim]")
-    if dtype is None:
-        _need(t.dtype in _TYPES, f"{name} must be float32, float16 or bfloat16")
-    else:
-        _need(t.dtype == dtype, f"{name} must be {str(dtype).replace('torch.', '')}")
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A [n, dim] tensor of values that lie next to each other in each row (a copy if they do not)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be CUDA tensor")
+    if t.ndim != 2:
+        raise ValueError(f"{name} must have shape [n, dim]")
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} asks for a gradient: the 8-bit rows have no backward pass (use torch.no_grad())")
     n, dim = t.shape
-    _need(1 <= dim <= _native.CIRCUIT_INT8_MAX_DIM, f"dim must be in [1, {_native.CIRCUIT_INT8_MAX_DIM}]")
-    if (dim > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < dim):
+    if not 1 <= dim <= _MAX_DIM:
+        raise ValueError(f"dim must be in [1, {_MAX_DIM}]")
+    s0, s1 = t.stride()
+    if (s1 != 1 and dim > 1) or (s0 < dim and n > 1):
         return t.contiguous()
     return t
 
 
-def _stride(t: torch.Tensor) -> int:
-    """Elements from one row to the next (a single row may carry any number)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _step(t: torch.Tensor) -> int:
+    """Elements from one row of a [n, dim] tensor to the next (a single row may carry any number)."""
+    n, dim = t.shape
+    s = t.stride(0)
+    return s if n > 1 or s > dim else dim
 
 
-def _padded(dim: int) -> int:
-    return (dim + 15) // 16 * 16
-
-
-def _alloc(n: int, dim: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
-    codes = torch.empty((n, _padded(dim)), dtype=torch.int8, device=device)
-    return (codes if codes.shape[1] == dim else codes[:, :dim]), torch.empty(n, dtype=torch.float32, device=device)
-
-
-def _ids(t: torch.Tensor, name: str, device) -> torch.Tensor:
+def _ids(t: torch.Tensor, name: str, dev: int) -> torch.Tensor:
     _cuda(t, name)
-    _need(t.dtype in (torch.int32, torch.int64), f"{name} must be int32 or int64")
-    _need(t.device == device, f"{name} must be on {device}")
+    if t.dtype != torch.int64 and t.dtype != torch.int32:
+        raise ValueError(f"{name} must be int32 or int64")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on the rows' device")
     return t.contiguous()
 
 
-def _pair(codes, scales, name: str, writable: bool = False) -> None:
+def _pair(codes, scales, name: str) -> None:
     """Checks codes [n, dim] int8 and scales [n] float32 of one device."""
     _cuda(codes, name + " codes")
     _cuda(scales, name + " scales")
-    _need(codes.ndim == 2 and codes.dtype == torch.int8, f"{name} codes must be int8 of shape [n, dim]")
-    _need(scales.ndim == 1 and scales.dtype == torch.float32 and scales.shape[0] == codes.shape[0],
-          f"{name} scales must be float32 of shape [n]")
-    _need(scales.device == codes.device, f"{name} codes and scales must be on one device")
-    if writable:
-        _need(codes.shape[1] == 1 or codes.stride(1) == 1, f"{name} codes must be contiguous in each row")
-        _need(codes.shape[0] < 2 or codes.stride(0) >= codes.shape[1], f"{name} code rows must not overlap")
-        _need(scales.is_contiguous(), f"{name} scales must be contiguous")
+    if codes.ndim != 2 or codes.dtype != torch.int8:
+        raise ValueError(f"{name} codes must be int8 of shape [n, dim]")
+    if scales.ndim != 1 or scales.dtype != torch.float32 or scales.shape[0] != codes.shape[0]:
+        raise ValueError(f"{name} scales must be float32 of shape [n]")
+    if scales.get_device() != codes.get_device():
+        raise ValueError(f"{name} codes and scales must be on one device")
+    if not 1 <= codes.shape[1] <= _MAX_DIM:
+        raise ValueError(f"dim must be in [1, {_MAX_DIM}]")
 
 
-class _on:
-    """The tensor's device as the current one, and its current stream."""
-
-    __slots__ = ("device", "guard", "stream")
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.guard = None
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _target(t: torch.Tensor, name: str) -> None:
+    """Refuses an output whose rows overlap or are not contiguous."""
+    n, dim = t.shape
+    if (dim > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < dim):
+        raise ValueError(f"{name} must be contiguous in each row and its rows must not overlap")
 
 
 def _quantize(rows, residual, weight, norm, eps, slots, out):
     rows = _rows(rows, "rows")
+    dev = rows.get_device()
+    if dev != _device():
+        with torch.cuda.device(dev):
+            return _quantize(rows, residual, weight, norm, eps, slots, out)
     n, dim = rows.shape
-    dev = rows.device
     summed = None
+    res_ptr = res_step = sum_ptr = w_ptr = slot_ptr = None
+    w_type = slot_bytes = 0
     if residual is not None:
-        residual = _rows(residual, "residual", rows.dtype)
-        _need(residual.shape == rows.shape, "residual must have the shape of rows")
-        _need(residual.device == dev, f"residual must be on {dev}")
+        residual = _rows(residual, "residual")
+        if residual.shape != rows.shape or residual.dtype != rows.dtype or residual.get_device() != dev:
+            raise ValueError("residual must have the shape, type and device of rows")
+        summed = torch.empty((n, dim), dtype=rows.dtype, device=rows.device)
+        res_ptr, sum_ptr = residual.data_ptr(), summed.data_ptr()
+        res_step = _step(residual)
     if weight is not None:
         _cuda(weight, "weight")
-        _need(weight.dtype in (rows.dtype, torch.float32), "weight must be of the rows' type or float32")
-        _need(weight.shape == (dim,) and weight.device == dev, f"weight must have shape [dim] and be on {dev}")
+        if weight.dtype != rows.dtype and weight.dtype != torch.float32:
+            raise ValueError("weight must be of the rows' type or float32")
+        if weight.shape != (dim,) or weight.get_device() != dev:
+            raise ValueError("weight must have shape [dim] and be on the rows' device")
         if weight.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("weight asks for a gradient: the 8-bit rows have no backward pass (use torch.no_grad())")
         weight = weight.contiguous()
-    _need(0.0 <= eps < float("inf"), "eps must be finite and not negative")
+        w_ptr, w_type = weight.data_ptr(), _TYPES[weight.dtype]
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("eps must be finite and not negative")
     if slots is not None:
-        _need(out is not None, "slots need the store to write to as out=(codes, scales)")
-        slots = _ids(slots, "slots", dev)
-        _need(slots.shape == (n,), "slots must have shape [n]")
-    with _on(dev) as stream:
         if out is None:
-            codes, scales = _alloc(n, dim, dev)
-        else:
-            codes, scales = out
-            _pair(codes, scales, "out", writable=True)
-            _need(codes.device == dev, f"out must be on {dev}")
-            _need(codes.shape[1] == dim, "out must have the rows' dim")
-            _need(slots is not None or codes.shape[0] == n, "out must hold as many rows as there are (or give slots)")
-        if residual is not None:
-            summed = torch.empty((n, dim), dtype=rows.dtype, device=dev)
-        if n and codes.shape[0]:
-            rc = _native.lib().circuit_op_quantize_rows(
-                rows.data_ptr(), _TYPES[rows.dtype], n, dim, _stride(rows),
-                residual.data_ptr() if residual is not None else None,
-                _stride(residual) if residual is not None else 0,
-                weight.data_ptr() if weight is not None else None, _TYPES[weight.dtype] if weight is not None else 0,
-                norm, eps, summed.data_ptr() if summed is not None else None, dim,
-                slots.data_ptr() if slots is not None else None, slots.element_size() if slots is not None else 0,
-                codes.shape[0], codes.data_ptr(), _stride(codes), scales.data_ptr(), stream)
+            raise ValueError("slots need the store to write to as out=(codes, scales)")
+        slots = _ids(slots, "slots", dev)
+        if slots.shape != (n,):
+            raise ValueError("slots must have shape [n]")
+        slot_ptr, slot_bytes = slots.data_ptr(), slots.element_size()
+    if out is None:
+        capacity, step = n, (dim + 15) // 16 * 16
+        codes = torch.empty((n, step), dtype=torch.int8, device=rows.device)
+        scales = torch.empty(n, dtype=torch.float32, device=rows.device)
+        if step != dim:
+            codes = codes[:, :dim]
+    else:
+        codes, scales = out
+        _pair(codes, scales, "out")
+        _target(codes, "out codes")
+        if not scales.is_contiguous():
+            raise ValueError("out scales must be contiguous")
+        if codes.get_device() != dev:
+            raise ValueError("out must be on the rows' device")
+        capacity, step = codes.shape[0], _step(codes)
+        if codes.shape[1] != dim:
+            raise ValueError("out must have the rows' dim")
+        if slots is None and capacity != n:
+            raise ValueError("out must hold as many rows as there are (or give slots)")
+    if n and capacity:
+        rc = _native.lib().circuit_op_quantize_rows(
+            rows.data_ptr(), _TYPES[rows.dtype], n, dim, _step(rows), res_ptr, res_step or 0, w_ptr, w_type, norm, eps,
+            sum_ptr, dim, slot_ptr, slot_bytes, capacity, codes.data_ptr(), step, scales.data_ptr(), _stream(dev))
+        if rc:
             _native.check(rc, "quantize_rows")
-        elif summed is not None and n:
-            torch.add(rows, residual, out=summed)
+    elif n and summed is not None:  # a store without slots: nothing is written, the sum is still due
+        torch.add(rows, residual, out=summed)
     return codes, scales, summed
 
 
@@ -182,46 +186,48 @@ def dequantize_rows(codes: torch.Tensor, scales: torch.Tensor, ids: Optional[tor
     [*ids.shape, dim]; all rows without ids), rounded once to ``dtype``.  A negative id, as a search returns for a
     place without a result, gives zeros; an id past the last row gives NaN."""
     _pair(codes, scales, "rows'")
-    _need(dtype in _TYPES, "dtype must be float32, float16 or bfloat16")
+    if dtype not in _TYPES:
+        raise ValueError("dtype must be float32, float16 or bfloat16")
+    dev = codes.get_device()
+    if dev != _device():
+        with torch.cuda.device(dev):
+            return dequantize_rows(codes, scales, ids, dtype, out)
     rows, dim = codes.shape
-    dev = codes.device
-    _need(1 <= dim <= _native.CIRCUIT_INT8_MAX_DIM, f"dim must be in [1, {_native.CIRCUIT_INT8_MAX_DIM}]")
-    if (dim > 1 and codes.stride(1) != 1) or (rows > 1 and codes.stride(0) < dim):
+    s0, s1 = codes.stride()
+    if (s1 != 1 and dim > 1) or (s0 < dim and rows > 1):
         codes = codes.contiguous()
     scales = scales.contiguous()
+    n, shape, id_ptr, id_bytes = rows, (rows, dim), None, 0
     if ids is not None:
         ids = _ids(ids, "ids", dev)
-    shape = (rows if ids is None else ids.numel(), dim)
-    with _on(dev) as stream:
-        if out is None:
-            out = torch.empty(shape if ids is None else (*ids.shape, dim), dtype=dtype, device=dev)
-            flat = out
-        else:
-            _cuda(out, "out")
-            _need(out.dtype == dtype and out.device == dev and out.shape == shape,
-                  f"out must be of type dtype, of shape [{shape[0]}, {dim}], on {dev}")
-            _need((dim == 1 or out.stride(1) == 1) and (shape[0] < 2 or out.stride(0) >= dim),
-                  "out must be contiguous in each row and its rows must not overlap")
-            flat = out
-        if shape[0]:
-            rc = _native.lib().circuit_op_dequantize_rows(
-                codes.data_ptr(), _stride(codes), scales.data_ptr(), rows, dim,
-                ids.data_ptr() if ids is not None else None, ids.element_size() if ids is not None else 0, shape[0],
-                flat.data_ptr(), _TYPES[dtype], _stride(flat) if flat.ndim == 2 else dim, stream)
+        n, shape = ids.numel(), (*ids.shape, dim)
+        id_ptr, id_bytes = ids.data_ptr(), ids.element_size()
+    step = dim
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=codes.device)
+    else:
+        _cuda(out, "out")
+        if out.dtype != dtype or out.get_device() != dev or out.shape != (n, dim):
+            raise ValueError(f"out must be of type dtype, of shape [{n}, {dim}], on the rows' device")
+        _target(out, "out")
+        step = _step(out)
+    if n:
+        rc = _native.lib().circuit_op_dequantize_rows(codes.data_ptr(), _step(codes), scales.data_ptr(), rows, dim,
+                                                      id_ptr, id_bytes, n, out.data_ptr(), _TYPES[dtype], step,
+                                                      _stream(dev))
+        if rc:
             _native.check(rc, "dequantize_rows")
     return out
 
 
 def _code_rows(codes: torch.Tensor) -> torch.Tensor:
-    """Codes as int8_scores reads them: rows on 16 bytes, their padding inside the storage (a padded copy if not)."""
+    """Codes as the products read them: rows on 16 bytes, their padding inside the storage (a padded copy if not)."""
     n, dim = codes.shape
-    stride = _stride(codes)
-    if ((dim == 1 or codes.stride(1) == 1) and stride % 16 == 0 and stride >= _padded(dim)
-            and codes.data_ptr() % 16 == 0
-            and codes.storage_offset() + (n - 1) * stride + _padded(dim) <= codes.untyped_storage().nbytes()):
+    step, padded = _step(codes), (dim + 15) // 16 * 16
+    if ((dim == 1 or codes.stride(1) == 1) and step % 16 == 0 and step >= padded and codes.data_ptr() % 16 == 0
+            and (padded == dim or codes.storage_offset() + (n - 1) * step + padded <= codes.untyped_storage().nbytes())):
         return codes
-    new = torch.empty((n, _padded(dim)), dtype=torch.int8, device=codes.device)[:, :dim]
-    return new.copy_(codes)
+    return torch.empty((n, padded), dtype=torch.int8, device=codes.device)[:, :dim].copy_(codes)
 
 
 def int8_scores(query_codes: torch.Tensor, query_scales: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -234,34 +240,42 @@ def int8_scores(query_codes: torch.Tensor, query_scales: torch.Tensor, codes: to
     those of quantize_rows and Int8Rows never are."""
     _pair(query_codes, query_scales, "query")
     _pair(codes, scales, "rows'")
-    _need(dtype in _TYPES, "dtype must be float32, float16 or bfloat16")
+    if dtype not in _TYPES:
+        raise ValueError("dtype must be float32, float16 or bfloat16")
+    dev = codes.get_device()
+    if query_codes.get_device() != dev:
+        raise ValueError("queries must be on the rows' device")
+    if dev != _device():
+        with torch.cuda.device(dev):
+            return int8_scores(query_codes, query_scales, codes, scales, bias, dtype, out)
     nq, dim = query_codes.shape
     n = codes.shape[0]
-    dev = codes.device
-    _need(codes.shape[1] == dim, "queries and rows must have one dim")
-    _need(1 <= dim <= _native.CIRCUIT_INT8_MAX_DIM, f"dim must be in [1, {_native.CIRCUIT_INT8_MAX_DIM}]")
-    _need(nq <= _native.CIRCUIT_INT8_MAX_QUERIES, f"at most {_native.CIRCUIT_INT8_MAX_QUERIES} queries a call")
-    _need(query_codes.device == dev, f"queries must be on {dev}")
+    if codes.shape[1] != dim:
+        raise ValueError("queries and rows must have one dim")
+    if nq > _native.CIRCUIT_INT8_MAX_QUERIES:
+        raise ValueError(f"at most {_native.CIRCUIT_INT8_MAX_QUERIES} queries a call")
+    bias_ptr = None
     if bias is not None:
         _cuda(bias, "bias")
-        _need(bias.dtype == torch.float32 and bias.shape == (n,) and bias.device == dev,
-              f"bias must be float32 of shape [n] on {dev}")
+        if bias.dtype != torch.float32 or bias.shape != (n,) or bias.get_device() != dev:
+            raise ValueError("bias must be float32 of shape [n] on the rows' device")
         bias = bias.contiguous()
-    with _on(dev) as stream:
-        if out is None:
-            out = torch.empty((nq, n), dtype=dtype, device=dev)
-        else:
-            _cuda(out, "out")
-            _need(out.dtype == dtype and out.shape == (nq, n) and out.device == dev,
-                  f"out must be of type dtype, of shape [{nq}, {n}], on {dev}")
-            _need((n < 2 or out.stride(1) == 1) and (nq < 2 or out.stride(0) >= n),
-                  "out must be contiguous in each row and its rows must not overlap")
-        if nq and n:
-            query_codes, codes = _code_rows(query_codes), _code_rows(codes)
-            query_scales, scales = query_scales.contiguous(), scales.contiguous()
-            rc = _native.lib().circuit_op_int8_scores(
-                query_codes.data_ptr(), _stride(query_codes), query_scales.data_ptr(), nq, codes.data_ptr(),
-                _stride(codes), scales.data_ptr(), n, dim, bias.data_ptr() if bias is not None else None,
-                out.data_ptr(), _TYPES[dtype], _stride(out), stream)
+        bias_ptr = bias.data_ptr()
+    step = n
+    if out is None:
+        out = torch.empty((nq, n), dtype=dtype, device=codes.device)
+    else:
+        _cuda(out, "out")
+        if out.dtype != dtype or out.shape != (nq, n) or out.get_device() != dev:
+            raise ValueError(f"out must be of type dtype, of shape [{nq}, {n}], on the rows' device")
+        _target(out, "out")
+        step = _step(out)
+    if nq and n:
+        query_codes, codes = _code_rows(query_codes), _code_rows(codes)
+        query_scales, scales = query_scales.contiguous(), scales.contiguous()
+        rc = _native.lib().circuit_op_int8_scores(
+            query_codes.data_ptr(), _step(query_codes), query_scales.data_ptr(), nq, codes.data_ptr(), _step(codes),
+            scales.data_ptr(), n, dim, bias_ptr, out.data_ptr(), _TYPES[dtype], step, _stream(dev))
+        if rc:
             _native.check(rc, "int8_scores")
     return out
