@@ -16,28 +16,35 @@
 namespace cb {
 namespace i8 {
 
-// ---------------------------------------------------------------- reductions over the G threads of a row
+// ---------------------------------------------------------------- helpers
+// Maximum of magnitudes that keeps a NaN (fmaxf would drop it).
+__device__ __forceinline__ float max_abs_nan(float m, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+  return r;
+}
+
 struct RowSums {
-  float top, low;  // max |u| as the unevaluated sum top + low (top = the rounded product)
+  float top, low;  // max |u| as the unevaluated sum top + low (top: the rounded product); top NaN or inf: a bad row
   float ss;        // sum of v^2
-  int bad;         // some u is not finite
 };
-// (top, low) of two candidates: the larger real number.
+// (top, low) of two candidates: the larger real number; a NaN stays.
 __device__ __forceinline__ void raise(float& top, float& low, float t, float l) {
-  if (t > top || (t == top && l > low)) {
+  if (t > top || (t == top && l > low) || t != t) {
     top = t;
     low = l;
   }
 }
-template <int G>
+// Over the G threads of a row.
+template <int G, bool LOW, bool SS>
 __device__ __forceinline__ RowSums reduce(RowSums r) {
   constexpr int W = G < 32 ? G : 32;
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1) {
-    const float t = __shfl_xor_sync(FULL_MASK, r.top, o), l = __shfl_xor_sync(FULL_MASK, r.low, o);
-    raise(r.top, r.low, t, l);
-    r.ss += __shfl_xor_sync(FULL_MASK, r.ss, o);
-    r.bad |= __shfl_xor_sync(FULL_MASK, r.bad, o);
+    const float t = __shfl_xor_sync(FULL_MASK, r.top, o);
+    if constexpr (LOW) raise(r.top, r.low, t, __shfl_xor_sync(FULL_MASK, r.low, o));
+    else r.top = max_abs_nan(r.top, t);
+    if constexpr (SS) r.ss += __shfl_xor_sync(FULL_MASK, r.ss, o);
   }
   if constexpr (G > 32) {
     __shared__ RowSums part[G / 32];
@@ -47,19 +54,21 @@ __device__ __forceinline__ RowSums reduce(RowSums r) {
     r = part[0];
 #pragma unroll
     for (int w = 1; w < G / 32; ++w) {
-      raise(r.top, r.low, part[w].top, part[w].low);
-      r.ss += part[w].ss;
-      r.bad |= part[w].bad;
+      if constexpr (LOW) raise(r.top, r.low, part[w].top, part[w].low);
+      else r.top = max_abs_nan(r.top, part[w].top);
+      if constexpr (SS) r.ss += part[w].ss;
     }
   }
   return r;
 }
 
-// The code of u = v * w: rint(127 u / a) of the real quotient, ties to even.
-// t = u * (127 / a) in 32 bits is within 3.1e-5 of 127 u / a (four roundings of
-// relative size 2^-24 at |t| <= 127), so its nearest integer is the code unless
-// t lies within 6e-5 of a half; there (0.012 % of the values) the quotient is
-// taken in 64 bits, where v * w is exact.
+// Codes.  With inv = 127 / top in 32 bits, one FMA adds u * inv to 1.5 * 2^23:
+// the sum's low byte is the nearest integer n, and u * inv - n (a second FMA) its
+// remainder.  u, inv and top are off by 2^-24 of their size each, so u * inv is
+// within 127 * 3 * 2^-24 < 2.3e-5 of the real quotient and n is its nearest
+// integer unless the remainder is within 6e-5 of a half; there (0.012 % of the
+// values) the quotient is taken in 64 bits, where v * w is exact.
+constexpr float ROUNDER = 12582912.f;
 constexpr float NEAR_HALF = 0.5f - 6e-5f;
 __device__ __forceinline__ int code_near_half(float v, float w, double a) {
   return (int)rint((double)v * (double)w * 127.0 / a);
@@ -76,8 +85,8 @@ struct QuantizeParams {
   int64_t n, x_stride, res_stride, sum_stride, code_stride, capacity;
   int d;
   int w_f32;            // the weight is fp32 (else of the row's type)
-  int norm;             // 0: scale a / 127; else divided by sqrt(ss * inv_n + eps)
-  float inv_n, eps;
+  int inexact;          // a product of value and weight may need more than 24 bits
+  float inv_n, eps;     // norm: the scale is divided by sqrt(ss * inv_n + eps)
   int slot64, claimed;  // slots are int64; slots were claimed by k_claim_slots
   int wide_in, wide_out;
 };
@@ -102,160 +111,196 @@ __global__ void k_claim_slots(const void* slots, int slot64, int64_t n, int64_t 
   if (s >= 0 && s < capacity) atomicMax(reinterpret_cast<uint32_t*>(scales + s), claim_tag(i));
 }
 
-// G threads a row (a warp, or a block of G), the row in NV 16-byte vectors of
-// registers a thread: it is read once and never again.  FULL: with residual,
-// weight and norm as the parameters say; otherwise the plain quantisation.
-constexpr int quantize_threads(int G) { return G == 32 ? 256 : G; }
+constexpr int quantize_threads(int G) { return G <= 32 ? 256 : G; }
 
+// G threads a row (8 lanes, a warp, or a block), the row in NV 16-byte vectors a
+// thread: it is read once.  FULL: with residual, weight and norm as the
+// parameters say; otherwise the plain quantisation.  Memory-bound by design: per
+// value one NaN-keeping maximum (and one FMA for the squares) before the row's
+// reduction, two FMAs, an add and a maximum after it.
 template <typename T, int G, int NV, bool FULL>
 __global__ void __launch_bounds__(quantize_threads(G)) k_quantize_rows(QuantizeParams P) {
   constexpr int V = RowType<T>::V;
   const int lane = threadIdx.x % G;
   const int64_t row = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) / G;
-  const bool live = row < P.n;  // G = 32: whole warps; G > 32: one row a block, always live
-  if (!live) return;
-  const int d = P.d;
+  const bool live = row < P.n;
+  if constexpr (G >= 32) {
+    if (!live) return;  // whole warps; with fewer lanes a row the others of the warp need the shuffles
+  }
+  const int d = live ? P.d : 0;
 
-  // where the row goes; of equal slots the last row's write stays
-  int64_t dst = row;
+  // where the row goes (-1: nowhere); of equal slots the last row's write stays
+  int64_t dst = live ? row : -1;
   if (P.slots) {
-    dst = slot_at(P.slots, P.slot64, row);
+    dst = live ? slot_at(P.slots, P.slot64, row) : -1;
     bool mine = dst >= 0 && dst < P.capacity;
-    if (mine && P.claimed) {
-      mine = __ldcg(reinterpret_cast<const uint32_t*>(P.scales + dst)) == claim_tag(row);
-    } else if (mine) {
-      int later = 0;
-      for (int64_t j = row + 1 + lane; j < P.n; j += G) later |= slot_at(P.slots, P.slot64, j) == dst;
-      if constexpr (G > 32) later = __syncthreads_or(later);
-      else later = __any_sync(FULL_MASK, later);
-      mine = !later;
-    }
-    if constexpr (G > 32) {
-      if (P.claimed) mine = __syncthreads_and(mine);  // every thread has read the claim before it is overwritten
+    if (P.claimed) {
+      mine = mine && __ldcg(reinterpret_cast<const uint32_t*>(P.scales + dst)) == claim_tag(row);
+      // every thread has read the claim before the row's scale overwrites it
+      if constexpr (G > 32) __syncthreads();
+      else __syncwarp();
     } else {
-      mine = __all_sync(FULL_MASK, mine);
+      int later = 0;
+      if (mine)
+        for (int64_t j = row + 1 + lane; j < P.n; j += G) later |= slot_at(P.slots, P.slot64, j) == dst;
+      if constexpr (G > 32) {
+        later = __syncthreads_or(later);
+      } else {
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) later |= __shfl_xor_sync(FULL_MASK, later, o);
+      }
+      mine = mine && !later;
     }
     if (!mine) dst = -1;
-    if (dst < 0 && !(FULL && P.res)) return;
+    if constexpr (G >= 32) {
+      if (dst < 0 && !(FULL && P.res)) return;
+    }
   }
 
-  const T* x = reinterpret_cast<const T*>(P.x) + row * P.x_stride;
+  const T* x = reinterpret_cast<const T*>(P.x) + (live ? row : 0) * P.x_stride;
   Vec<T> v[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) v[k] = load_vec(x, (k * G + lane) * V, d, P.wide_in & 1);
+  RowSums r{0.f, 0.f, 0.f};
+  float u[FULL ? NV : 1][FULL ? V : 1];  // v * w, rounded
   if constexpr (FULL) {
     if (P.res) {
-      const T* r = reinterpret_cast<const T*>(P.res) + row * P.res_stride;
-      T* s = reinterpret_cast<T*>(P.sum) + row * P.sum_stride;
+      const T* res = reinterpret_cast<const T*>(P.res) + (live ? row : 0) * P.res_stride;
+      Vec<T> b[NV];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) b[k] = load_vec(res, (k * G + lane) * V, d, P.wide_in & 2);
+      T* sum = reinterpret_cast<T*>(P.sum) + (live ? row : 0) * P.sum_stride;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const Vec<T> b = load_vec(r, (k * G + lane) * V, d, P.wide_in & 2);
         // the sum is kept in the row's type, as the next layer reads it; the
         // norm and the codes are those of the kept value
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          v[k].e[i] = RowType<T>::put(RowType<T>::get(v[k].e[i]) + RowType<T>::get(b.e[i]));
-        store_vec(s, (k * G + lane) * V, d, P.wide_in & 4, v[k]);
+          v[k].e[i] = RowType<T>::put(RowType<T>::get(v[k].e[i]) + RowType<T>::get(b[k].e[i]));
+        store_vec(sum, (k * G + lane) * V, d, P.wide_in & 4, v[k]);
       }
     }
-  }
-
-  float wt[FULL ? NV : 1][FULL ? V : 1];
-  if constexpr (FULL) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * G + lane) * V;
+      float w[V];
       if (!P.w) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) wt[k][i] = 1.f;
+        for (int i = 0; i < V; ++i) w[i] = 1.f;
       } else if (P.w_f32) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) wt[k][i] = c + i < d ? __ldg(reinterpret_cast<const float*>(P.w) + c + i) : 0.f;
+        for (int i = 0; i < V; ++i) w[i] = c + i < d ? __ldg(reinterpret_cast<const float*>(P.w) + c + i) : 0.f;
       } else {
         const Vec<T> b = load_vec(reinterpret_cast<const T*>(P.w), c, d, P.wide_in & 8);
 #pragma unroll
-        for (int i = 0; i < V; ++i) wt[k][i] = RowType<T>::get(b.e[i]);
+        for (int i = 0; i < V; ++i) w[i] = RowType<T>::get(b.e[i]);
       }
-    }
-  }
-
-  RowSums r{0.f, 0.f, 0.f, 0};
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float e = RowType<T>::get(v[k].e[i]);
-      float a = fabsf(e);
-      if constexpr (FULL) {
+      for (int i = 0; i < V; ++i) {
+        const float e = RowType<T>::get(v[k].e[i]);
         r.ss = fmaf(e, e, r.ss);
-        const float aw = fabsf(wt[k][i]), p = a * aw;
-        if (p >= r.top) raise(r.top, r.low, p, fmaf(a, aw, -p));  // fma gives the product's rounding error
-        a = p;
-      } else {
-        r.top = fmaxf(r.top, a);
+        u[k][i] = e * w[i];
       }
-      r.bad |= !(a <= FLT_MAX);
+      if (P.inexact) {  // an fp32 factor: the FMA gives the product's rounding error
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float p = fabsf(u[k][i]);
+          if (!(p < r.top)) raise(r.top, r.low, p, fmaf(fabsf(RowType<T>::get(v[k].e[i])), fabsf(w[i]), -p));
+        }
+      } else {  // 8- or 11-bit factors: their product is exact
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.top = max_abs_nan(r.top, u[k][i]);
+      }
     }
-  r = reduce<G>(r);
+    r = P.inexact ? reduce<G, true, true>(r) : reduce<G, false, true>(r);
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) r.top = max_abs_nan(r.top, RowType<T>::get(v[k].e[i]));
+    r = reduce<G, false, false>(r);
+  }
+  const bool bad = !(r.top <= FLT_MAX);
 
   float scale = r.top / 127.f;
-  if (FULL && P.norm && r.top > 0.f && !r.bad) {
-    if (r.ss > 1e-25f && r.ss < FLT_MAX) {
-      scale /= sqrtf(fmaf(r.ss, P.inv_n, P.eps));
-    } else {
+  if constexpr (FULL) {
+    const bool odd = r.top > 0.f && !bad && !(r.ss > 1e-25f && r.ss < FLT_MAX);
+    if (r.top > 0.f && !bad && !odd) scale /= sqrtf(fmaf(r.ss, P.inv_n, P.eps));
+    if (G >= 32 ? odd : __any_sync(FULL_MASK, odd)) {
       // the squares left the range of 32 bits: sum them again as (v 2^-e)^2
-      RowSums m{0.f, 0.f, 0.f, 0};
+      RowSums m{0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) m.top = fmaxf(m.top, fabsf(RowType<T>::get(v[k].e[i])));
-      m = reduce<G>(m);
-      const int e = ilogbf(m.top);
+        for (int i = 0; i < V; ++i) m.top = max_abs_nan(m.top, RowType<T>::get(v[k].e[i]));
+      m = reduce<G, false, false>(m);
+      const int e = odd ? ilogbf(m.top) : 0;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float s = ldexpf(RowType<T>::get(v[k].e[i]), -e);
-          m.ss = fmaf(s, s, m.ss);
+          const float q = ldexpf(RowType<T>::get(v[k].e[i]), -e);
+          m.ss = fmaf(q, q, m.ss);
         }
-      m = reduce<G>(m);
-      const double mean = ldexp((double)m.ss * (double)P.inv_n, 2 * e) + (double)P.eps;
-      scale = (float)((double)r.top / 127.0 / sqrt(mean));
+      m = reduce<G, false, true>(m);
+      if (odd) {
+        const double mean = ldexp((double)m.ss * (double)P.inv_n, 2 * e) + (double)P.eps;
+        scale = (float)((double)r.top / 127.0 / sqrt(mean));
+      }
     }
   }
-  if (dst < 0) return;
-  if (r.bad) scale = __uint_as_float(0x7fffffffu);  // a NaN without the sign that marks claims
+  if (dst < 0) return;  // nothing below needs the other lanes
+  if (bad) scale = __uint_as_float(0x7fffffffu);  // a NaN without the sign that marks claims
   if (lane == 0) P.scales[dst] = scale;
 
-  // tiny rows are brought into range by a power of two, so 127 / a stays finite
-  const float pre = r.top < 1e-18f ? 1.2089258196146292e24f : 1.f;  // 2^80
-  const float inv = r.bad || r.top == 0.f ? 0.f : 127.f / (r.top * pre);
-  const double a = (double)r.top + (double)r.low;
   int8_t* out = P.codes + dst * P.code_stride;
+  // tiny rows are brought into range by a power of two, so 127 / top stays finite
+  const float pre = r.top < 1e-18f ? 1.2089258196146292e24f : 1.f;  // 2^80
+  const float inv = bad || r.top == 0.f ? 0.f : 127.f / (r.top * pre);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    union {
-      int8_t b[V];
-      uint32_t w[V / 4];
-    } q;
+    const int c = (k * G + lane) * V;
+    uint32_t n[V];
+    float off = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float e = RowType<T>::get(v[k].e[i]);
-      float w = 1.f;
-      if constexpr (FULL) w = wt[k][i];
-      const float t = e * w * pre * inv, n = rintf(t);
-      int code = (int)n;
-      if (fabsf(t - n) > NEAR_HALF) code = code_near_half(e, w, a);
-      q.b[i] = r.bad ? (int8_t)0 : (int8_t)code;
+      float t;
+      if constexpr (FULL) t = u[k][i];
+      else t = RowType<T>::get(v[k].e[i]);
+      if (pre != 1.f) t *= pre;
+      const float big = fmaf(t, inv, ROUNDER);
+      off = fmaxf(off, fabsf(fmaf(t, inv, ROUNDER - big)));
+      n[i] = __float_as_uint(big);
     }
-    const int c = (k * G + lane) * V;
+    if (off > NEAR_HALF) {
+      const double a = (double)r.top + (double)r.low;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float w = 1.f;
+        if constexpr (FULL) {
+          if (P.w && c + i < d)
+            w = P.w_f32 ? __ldg(reinterpret_cast<const float*>(P.w) + c + i)
+                        : RowType<T>::get(reinterpret_cast<const T*>(P.w)[c + i]);
+        }
+        n[i] = (uint32_t)code_near_half(RowType<T>::get(v[k].e[i]), w, a);
+      }
+    }
+    if (bad) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) n[i] = 0;
+    }
+    uint32_t q[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      q[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040),
+                         0x5410);
     if (P.wide_out && c + V <= d) {
-      if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + c) = q.w[0];
-      else *reinterpret_cast<uint2*>(out + c) = make_uint2(q.w[0], q.w[1]);
+      if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + c) = q[0];
+      else *reinterpret_cast<uint2*>(out + c) = make_uint2(q[0], q[1]);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (c + i < d) out[c + i] = q.b[i];
+        if (c + i < d) out[c + i] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
     }
   }
 }
@@ -270,54 +315,68 @@ struct ReadParams {
   int d, id64, wide_in, wide_out;
 };
 
-// A warp a row: 16 bytes of output a lane and step.  An id below 0 is an empty
-// place (zeros), one past the store a mistake (NaN).
-template <typename T>
+// A warp reads R rows together (their loads are in flight at once), 16 bytes of
+// output a lane, row and step.  An id below 0 is an empty place (zeros), one past
+// the store a mistake (NaN).
+template <typename T, int R>
 __global__ void __launch_bounds__(256) k_dequantize_rows(ReadParams P) {
   constexpr int V = RowType<T>::V;
   const int lane = threadIdx.x & 31;
-  const int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-  if (i >= P.n) return;
-  const int64_t id = P.ids ? slot_at(P.ids, P.id64, i) : i;
-  const bool known = id >= 0 && id < P.rows;
-  const float scale = known ? __ldg(P.scales + id) : id < 0 ? 0.f : __uint_as_float(0x7fffffffu);
-  const int8_t* in = P.codes + (known ? id : 0) * P.code_stride;
-  T* out = reinterpret_cast<T*>(P.out) + i * P.out_stride;
-  for (int c = lane * V; c < P.d; c += 32 * V) {
-    union {
-      int8_t b[V];
-      uint32_t w[V / 4];
-    } q;
+  const int64_t i0 = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) / 32 * R;
+  if (i0 >= P.n) return;
+  bool known[R];
+  float scale[R];
+  const int8_t* in[R];
 #pragma unroll
-    for (int k = 0; k < V / 4; ++k) q.w[k] = 0;
-    if (known) {
+  for (int r = 0; r < R; ++r) {
+    int64_t id = -1;
+    if (i0 + r < P.n) id = P.ids ? slot_at(P.ids, P.id64, i0 + r) : i0 + r;
+    known[r] = id >= 0 && id < P.rows;
+    scale[r] = known[r] ? __ldg(P.scales + id) : id < 0 ? 0.f : __uint_as_float(0x7fffffffu);
+    in[r] = P.codes + (known[r] ? id : 0) * P.code_stride;
+  }
+  for (int c = lane * V; c < P.d; c += 32 * V) {
+    uint32_t w[R][V / 4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) w[r][k] = 0;
+      if (!known[r]) continue;
       if (P.wide_in && c + V <= P.d) {
         if constexpr (V == 4) {
-          q.w[0] = __ldg(reinterpret_cast<const uint32_t*>(in + c));
+          w[r][0] = __ldg(reinterpret_cast<const uint32_t*>(in[r] + c));
         } else {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(in + c));
-          q.w[0] = w.x;
-          q.w[1] = w.y;
+          const uint2 b = __ldg(reinterpret_cast<const uint2*>(in[r] + c));
+          w[r][0] = b.x;
+          w[r][1] = b.y;
         }
       } else {
 #pragma unroll
         for (int k = 0; k < V; ++k)
-          if (c + k < P.d) q.b[k] = __ldg(in + c + k);
+          if (c + k < P.d) w[r][k / 4] |= (uint32_t)(uint8_t)__ldg(in[r] + c + k) << (8 * (k % 4));
       }
     }
-    Vec<T> v;
 #pragma unroll
-    for (int k = 0; k < V; ++k) v.e[k] = RowType<T>::put((float)q.b[k] * scale);  // the value's one rounding
-    store_vec(out, c, P.d, P.wide_out, v);
+    for (int r = 0; r < R; ++r) {
+      if (i0 + r >= P.n) break;
+      Vec<T> v;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        // code + 128 in the low byte of 2^23, less 2^23 + 128: the code as a float
+        const uint32_t biased = w[r][k / 4] ^ 0x80808080u;
+        const float code = __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7540 | (k % 4))) - 8388736.f;
+        v.e[k] = RowType<T>::put(code * scale[r]);  // the value's one rounding
+      }
+      store_vec(reinterpret_cast<T*>(P.out) + (i0 + r) * P.out_stride, c, P.d, P.wide_out, v);
+    }
   }
 }
 
 // ---------------------------------------------------------------- host side
 template <typename T, int G, int NV, bool FULL>
 static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
-  constexpr int threads = quantize_threads(G);
-  const int64_t blocks = G == 32 ? (P.n + 7) / 8 : P.n;
-  k_quantize_rows<T, G, NV, FULL><<<(unsigned)blocks, threads, 0, st>>>(P);
+  constexpr int threads = quantize_threads(G), rows = threads / G;
+  k_quantize_rows<T, G, NV, FULL><<<(unsigned)((P.n + rows - 1) / rows), threads, 0, st>>>(P);
 }
 template <typename T, int G, bool FULL>
 static void quantize_nv(const QuantizeParams& P, int vectors, cudaStream_t st) {
@@ -328,14 +387,26 @@ static void quantize_nv(const QuantizeParams& P, int vectors, cudaStream_t st) {
   else if (G < 512 || RowType<T>::V == 8 || nv <= 4) launch_quantize<T, G, 4, FULL>(P, st);
   else if constexpr (G == 512 && RowType<T>::V == 4) launch_quantize<T, G, 8, FULL>(P, st);
 }
-// Threads a row: a warp while it holds the row in at most 4 vectors a lane,
-// then a block of 128, then of 512 (up to 8 vectors for 16,384 fp32 values).
+// Threads a row: 8 lanes while they hold the row in at most 4 vectors each, then
+// a warp, a block of 128 and a block of 512 (up to 8 vectors: 16,384 fp32 values).
 template <typename T, bool FULL>
 static void quantize(const QuantizeParams& P, cudaStream_t st) {
   const int vectors = (P.d + RowType<T>::V - 1) / RowType<T>::V;
-  if (vectors <= 32 * 4) quantize_nv<T, 32, FULL>(P, vectors, st);
+  if (vectors <= 8 * 4) quantize_nv<T, 8, FULL>(P, vectors, st);
+  else if (vectors <= 32 * 4) quantize_nv<T, 32, FULL>(P, vectors, st);
   else if (vectors <= 128 * 4) quantize_nv<T, 128, FULL>(P, vectors, st);
   else quantize_nv<T, 512, FULL>(P, vectors, st);
+}
+
+static void dequantize(const ReadParams& P, int dtype, cudaStream_t st) {
+  const bool many = P.n >= 148 * 32;
+  const unsigned blocks = (unsigned)(many ? (P.n + 31) / 32 : (P.n + 7) / 8);
+  if (dtype == CIRCUIT_F32) many ? k_dequantize_rows<float, 4><<<blocks, 256, 0, st>>>(P)
+                                 : k_dequantize_rows<float, 1><<<blocks, 256, 0, st>>>(P);
+  else if (dtype == CIRCUIT_F16) many ? k_dequantize_rows<__half, 4><<<blocks, 256, 0, st>>>(P)
+                                      : k_dequantize_rows<__half, 1><<<blocks, 256, 0, st>>>(P);
+  else many ? k_dequantize_rows<__nv_bfloat16, 4><<<blocks, 256, 0, st>>>(P)
+            : k_dequantize_rows<__nv_bfloat16, 1><<<blocks, 256, 0, st>>>(P);
 }
 
 }  // namespace i8
@@ -387,7 +458,7 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
   P.capacity = capacity;
   P.d = dim;
   P.w_f32 = weight && weight_dtype == CIRCUIT_F32;
-  P.norm = norm;
+  P.inexact = weight && (P.w_f32 || dtype == CIRCUIT_F32);
   P.inv_n = norm == CIRCUIT_NORM_RMS ? 1.f / (float)dim : 1.f;
   P.eps = eps;
   P.slot64 = slot_bytes == 8;
@@ -428,10 +499,7 @@ int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const f
   ReadParams P{codes, scales, ids, out, n, rows, code_stride, out_stride, dim, id_bytes == 8,
                (((uintptr_t)codes | (uintptr_t)code_stride) & 7) == 0, on16(out, out_stride * e)};
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned blocks = (unsigned)((n + 7) / 8);
-  if (dtype == CIRCUIT_F32) k_dequantize_rows<float><<<blocks, 256, 0, st>>>(P);
-  else if (dtype == CIRCUIT_F16) k_dequantize_rows<__half><<<blocks, 256, 0, st>>>(P);
-  else k_dequantize_rows<__nv_bfloat16><<<blocks, 256, 0, st>>>(P);
+  dequantize(P, dtype, st);
   return check(cudaGetLastError(), "dequantize_rows launch");
 }
 
