@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cstdint>
+#include <cstring>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -25,50 +26,86 @@ struct RowType<float> {
 };
 template <>
 struct RowType<__half> {
+  using Pair = __half2;
   static constexpr int V = 8;
   __device__ static float get(__half x) { return __half2float(x); }
   __device__ static __half put(float x) { return __float2half_rn(x); }
 };
 template <>
 struct RowType<__nv_bfloat16> {
+  using Pair = __nv_bfloat162;
   static constexpr int V = 8;
   __device__ static float get(__nv_bfloat16 x) { return __bfloat162float(x); }
   __device__ static __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
 };
 
-template <typename T>
-union Vec {
-  uint4 raw;
-  T e[RowType<T>::V];
-};
+// Maximum of magnitudes that keeps a NaN (fmaxf would drop it).
+__device__ __forceinline__ float max_abs_nan(float m, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+  return r;
+}
 
-// Elements [c, c + V) of a row of d elements: one 16-byte access where the row
-// allows it, else one access an element; zeros past the row's end.
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* row, int c, int d, bool wide) {
-  constexpr int V = RowType<T>::V;
-  Vec<T> v;
-  v.raw = make_uint4(0, 0, 0, 0);
-  if (wide && c + V <= d) {
-    v.raw = *reinterpret_cast<const uint4*>(row + c);
-  } else {
+// a += b, each sum rounded once to the row's type (pairs of 16-bit values in one instruction).
+template <typename T, int E>
+__device__ __forceinline__ void add_to(T (&a)[E], const T (&b)[E]) {
+  if constexpr (sizeof(T) == 4 || E == 1) {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (c + i < d) v.e[i] = row[c + i];
-  }
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ void store_vec(T* row, int c, int d, bool wide, const Vec<T>& v) {
-  constexpr int V = RowType<T>::V;
-  if (wide && c + V <= d) {
-    *reinterpret_cast<uint4*>(row + c) = v.raw;
+    for (int i = 0; i < E; ++i) a[i] = RowType<T>::put(RowType<T>::get(a[i]) + RowType<T>::get(b[i]));
   } else {
+    using P = typename RowType<T>::Pair;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (c + i < d) row[c + i] = v.e[i];
+    for (int i = 0; i < E; i += 2) {
+      const P s = __hadd2_rn(P{a[i], a[i + 1]}, P{b[i], b[i + 1]});
+      a[i] = s.x;
+      a[i + 1] = s.y;
+    }
   }
 }
+// top = max(top, |v|), a NaN stays.
+template <typename T, int E>
+__device__ __forceinline__ void raise_top(float& top, const T (&v)[E]) {
+  if constexpr (sizeof(T) == 4 || E == 1) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) top = max_abs_nan(top, RowType<T>::get(v[i]));
+  } else {
+    using P = typename RowType<T>::Pair;
+    P m = __habs2(P{v[0], v[1]});
+#pragma unroll
+    for (int i = 2; i < E; i += 2) m = __hmax2_nan(m, __habs2(P{v[i], v[i + 1]}));
+    top = max_abs_nan(max_abs_nan(top, RowType<T>::get(m.x)), RowType<T>::get(m.y));
+  }
+}
+
+// E elements of a row held by one thread: a 16-byte vector (rows on 16 bytes, of
+// whole vectors) or a single element (any row).
+template <typename T, int E>
+struct Vec {
+  T e[E];
+  // elements [c, c + E) of a row of d; zeros past its end
+  __device__ __forceinline__ static Vec load(const T* row, int c, int d) {
+    Vec v;
+    if constexpr (E == 1) {
+      v.e[0] = RowType<T>::put(0.f);
+      if (c < d) v.e[0] = row[c];
+    } else {
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (c < d) raw = *reinterpret_cast<const uint4*>(row + c);
+      memcpy(&v, &raw, 16);
+    }
+    return v;
+  }
+  __device__ __forceinline__ void store(T* row, int c, int d) const {
+    if (c >= d) return;
+    if constexpr (E == 1) {
+      row[c] = e[0];
+    } else {
+      uint4 raw;
+      memcpy(&raw, this, 16);
+      *reinterpret_cast<uint4*>(row + c) = raw;
+    }
+  }
+};
 
 // ---------------------------------------------------------------- host side
 inline int bad(const char* msg) {

@@ -17,13 +17,6 @@ namespace cb {
 namespace i8 {
 
 // ---------------------------------------------------------------- helpers
-// Maximum of magnitudes that keeps a NaN (fmaxf would drop it).
-__device__ __forceinline__ float max_abs_nan(float m, float x) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
-  return r;
-}
-
 struct RowSums {
   float top, low;  // max |u| as the unevaluated sum top + low (top: the rounded product); top NaN or inf: a bad row
   float ss;        // sum of v^2
@@ -62,14 +55,14 @@ __device__ __forceinline__ RowSums reduce(RowSums r) {
   return r;
 }
 
-// Codes.  With inv = 127 / top in 32 bits, one FMA adds u * inv to 1.5 * 2^23:
-// the sum's low byte is the nearest integer n, and u * inv - n (a second FMA) its
-// remainder.  u, inv and top are off by 2^-24 of their size each, so u * inv is
-// within 127 * 3 * 2^-24 < 2.3e-5 of the real quotient and n is its nearest
-// integer unless the remainder is within 6e-5 of a half; there (0.012 % of the
-// values) the quotient is taken in 64 bits, where v * w is exact.
+// Codes.  127 / top in 32 bits is taken a little up (hi) and down (lo), by 2^-21
+// of its size.  One FMA adds u * hi to 1.5 * 2^23, whose low byte is then the
+// nearest integer.  u, top and the division are off by 2^-24 of their size each and
+// hi and lo by another, so the real quotient lies between u * lo and u * hi: where
+// both give the same integer it is the code, where not (within 127 2^-21 = 6e-5 of
+// a half: 0.006 % of the values) the quotient is taken in 64 bits, in which v * w
+// is exact.
 constexpr float ROUNDER = 12582912.f;
-constexpr float NEAR_HALF = 0.5f - 6e-5f;
 __device__ __forceinline__ int code_near_half(float v, float w, double a) {
   return (int)rint((double)v * (double)w * 127.0 / a);
 }
@@ -88,7 +81,6 @@ struct QuantizeParams {
   int inexact;          // a product of value and weight may need more than 24 bits
   float inv_n, eps;     // norm: the scale is divided by sqrt(ss * inv_n + eps)
   int slot64, claimed;  // slots are int64; slots were claimed by k_claim_slots
-  int wide_in, wide_out;
 };
 
 __device__ __forceinline__ int64_t slot_at(const void* slots, int slot64, int64_t i) {
@@ -111,18 +103,85 @@ __global__ void k_claim_slots(const void* slots, int slot64, int64_t n, int64_t 
   if (s >= 0 && s < capacity) atomicMax(reinterpret_cast<uint32_t*>(scales + s), claim_tag(i));
 }
 
-constexpr int quantize_threads(int G) { return G <= 32 ? 256 : G; }
+constexpr int row_threads(int G) { return G <= 32 ? 256 : G; }
 
-// G threads a row (8 lanes, a warp, or a block), the row in NV 16-byte vectors a
-// thread: it is read once.  FULL: with residual, weight and norm as the
-// parameters say; otherwise the plain quantisation.  Memory-bound by design: per
-// value one NaN-keeping maximum (and one FMA for the squares) before the row's
-// reduction, two FMAs, an add and a maximum after it.
-template <typename T, int G, int NV, bool FULL>
-__global__ void __launch_bounds__(quantize_threads(G)) k_quantize_rows(QuantizeParams P) {
-  constexpr int V = RowType<T>::V;
+// The weights of elements [c, c + E) of a row.
+template <typename T, int E>
+__device__ __forceinline__ void load_weights(const QuantizeParams& P, int c, int d, float (&w)[E]) {
+  if (!P.w) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] = 1.f;
+  } else if (P.w_f32) {
+    constexpr int S = E == 1 ? 1 : 4;
+#pragma unroll
+    for (int i = 0; i < E; i += S) {
+      const auto b = Vec<float, S>::load(reinterpret_cast<const float*>(P.w), c + i, d);
+#pragma unroll
+      for (int j = 0; j < S; ++j) w[i + j] = b.e[j];
+    }
+  } else {
+    const auto b = Vec<T, E>::load(reinterpret_cast<const T*>(P.w), c, d);
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] = RowType<T>::get(b.e[i]);
+  }
+}
+
+// The codes n[i] & 255 of elements [c, c + E).
+template <int E>
+__device__ __forceinline__ void store_codes(int8_t* out, int c, const uint32_t (&n)[E], bool bad) {
+  if constexpr (E == 1) {
+    out[c] = bad ? 0 : (int8_t)n[0];
+  } else {
+    uint32_t q[E / 4];
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {
+      q[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040),
+                         0x5410);
+      if (bad) q[i] = 0;
+    }
+    if constexpr (E == 4) *reinterpret_cast<uint32_t*>(out + c) = q[0];
+    else *reinterpret_cast<uint2*>(out + c) = make_uint2(q[0], q[1]);
+  }
+}
+
+// Rare: the scale of a row whose squares leave the range of 32 bits, from
+// sum (v 2^-e)^2.  Each thread reads its own elements again (src: the row as
+// kept), in a rolled loop.
+template <typename T, int E, int G>
+__device__ __noinline__ float wide_range_scale(const T* src, int d, float top, float inv_n, float eps, bool odd) {
   const int lane = threadIdx.x % G;
-  const int64_t row = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) / G;
+  RowSums m{0.f, 0.f, 0.f};
+  for (int c = lane * E; c < d; c += G * E)
+    for (int i = 0; i < E; ++i) m.top = max_abs_nan(m.top, RowType<T>::get(src[c + i]));
+  m = reduce<G, false, false>(m);
+  const int e = odd ? ilogbf(m.top) : 0;
+  for (int c = lane * E; c < d; c += G * E)
+    for (int i = 0; i < E; ++i) {
+      const float q = ldexpf(RowType<T>::get(src[c + i]), -e);
+      m.ss = fmaf(q, q, m.ss);
+    }
+  m = reduce<G, false, true>(m);
+  return (float)((double)top / 127.0 / sqrt(ldexp((double)m.ss * (double)inv_n, 2 * e) + (double)eps));
+}
+
+// Rare: codes of elements [c, c + e) from the 64-bit quotient.
+template <typename T>
+__device__ __noinline__ void exact_codes(const QuantizeParams& P, const T* src, int8_t* out, int c, int e, double a) {
+  for (int i = c; i < c + e; ++i) {
+    float w = 1.f;
+    if (P.w) w = P.w_f32 ? reinterpret_cast<const float*>(P.w)[i] : RowType<T>::get(reinterpret_cast<const T*>(P.w)[i]);
+    out[i] = (int8_t)code_near_half(RowType<T>::get(src[i]), w, a);
+  }
+}
+
+// G threads a row (8 or 16 lanes, a warp, or a block), the row in NV vectors of E
+// elements a thread: it is read once.  FULL: with residual, weight and norm as the
+// parameters say; otherwise the plain quantisation.  With fewer lanes a row the
+// work of each row (reduction, addresses, scale) is shared by the rows of a warp.
+template <typename T, int E, int G, int NV, bool FULL>
+__global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_constant__ QuantizeParams P) {
+  const int lane = threadIdx.x % G;
+  const int64_t row = (int64_t)blockIdx.x * (row_threads(G) / G) + threadIdx.x / G;
   const bool live = row < P.n;
   if constexpr (G >= 32) {
     if (!live) return;  // whole warps; with fewer lanes a row the others of the warp need the shuffles
@@ -158,66 +217,46 @@ __global__ void __launch_bounds__(quantize_threads(G)) k_quantize_rows(QuantizeP
   }
 
   const T* x = reinterpret_cast<const T*>(P.x) + (live ? row : 0) * P.x_stride;
-  Vec<T> v[NV];
+  Vec<T, E> v[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) v[k] = load_vec(x, (k * G + lane) * V, d, P.wide_in & 1);
+  for (int k = 0; k < NV; ++k) v[k] = Vec<T, E>::load(x, (k * G + lane) * E, d);
   RowSums r{0.f, 0.f, 0.f};
-  float u[FULL ? NV : 1][FULL ? V : 1];  // v * w, rounded
   if constexpr (FULL) {
     if (P.res) {
       const T* res = reinterpret_cast<const T*>(P.res) + (live ? row : 0) * P.res_stride;
-      Vec<T> b[NV];
-#pragma unroll
-      for (int k = 0; k < NV; ++k) b[k] = load_vec(res, (k * G + lane) * V, d, P.wide_in & 2);
       T* sum = reinterpret_cast<T*>(P.sum) + (live ? row : 0) * P.sum_stride;
+      Vec<T, E> b[NV];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) b[k] = Vec<T, E>::load(res, (k * G + lane) * E, d);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         // the sum is kept in the row's type, as the next layer reads it; the
         // norm and the codes are those of the kept value
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          v[k].e[i] = RowType<T>::put(RowType<T>::get(v[k].e[i]) + RowType<T>::get(b[k].e[i]));
-        store_vec(sum, (k * G + lane) * V, d, P.wide_in & 4, v[k]);
+        add_to<T, E>(v[k].e, b[k].e);
+        v[k].store(sum, (k * G + lane) * E, d);
       }
+      x = sum;
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * G + lane) * V;
-      float w[V];
-      if (!P.w) {
+      float w[E];
+      load_weights<T, E>(P, (k * G + lane) * E, d, w);
 #pragma unroll
-        for (int i = 0; i < V; ++i) w[i] = 1.f;
-      } else if (P.w_f32) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) w[i] = c + i < d ? __ldg(reinterpret_cast<const float*>(P.w) + c + i) : 0.f;
-      } else {
-        const Vec<T> b = load_vec(reinterpret_cast<const T*>(P.w), c, d, P.wide_in & 8);
-#pragma unroll
-        for (int i = 0; i < V; ++i) w[i] = RowType<T>::get(b.e[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float e = RowType<T>::get(v[k].e[i]);
+      for (int i = 0; i < E; ++i) {
+        const float e = RowType<T>::get(v[k].e[i]), u = e * w[i];
         r.ss = fmaf(e, e, r.ss);
-        u[k][i] = e * w[i];
-      }
-      if (P.inexact) {  // an fp32 factor: the FMA gives the product's rounding error
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float p = fabsf(u[k][i]);
-          if (!(p < r.top)) raise(r.top, r.low, p, fmaf(fabsf(RowType<T>::get(v[k].e[i])), fabsf(w[i]), -p));
+        if (P.inexact) {  // an fp32 factor: the FMA gives the product's rounding error
+          const float p = fabsf(u);
+          if (!(p < r.top)) raise(r.top, r.low, p, fmaf(fabsf(e), fabsf(w[i]), -p));
+        } else {  // 8- or 11-bit factors: their product is exact
+          r.top = max_abs_nan(r.top, u);
         }
-      } else {  // 8- or 11-bit factors: their product is exact
-#pragma unroll
-        for (int i = 0; i < V; ++i) r.top = max_abs_nan(r.top, u[k][i]);
       }
     }
     r = P.inexact ? reduce<G, true, true>(r) : reduce<G, false, true>(r);
   } else {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) r.top = max_abs_nan(r.top, RowType<T>::get(v[k].e[i]));
+    for (int k = 0; k < NV; ++k) raise_top<T, E>(r.top, v[k].e);
     r = reduce<G, false, false>(r);
   }
   const bool bad = !(r.top <= FLT_MAX);
@@ -227,26 +266,8 @@ __global__ void __launch_bounds__(quantize_threads(G)) k_quantize_rows(QuantizeP
     const bool odd = r.top > 0.f && !bad && !(r.ss > 1e-25f && r.ss < FLT_MAX);
     if (r.top > 0.f && !bad && !odd) scale /= sqrtf(fmaf(r.ss, P.inv_n, P.eps));
     if (G >= 32 ? odd : __any_sync(FULL_MASK, odd)) {
-      // the squares left the range of 32 bits: sum them again as (v 2^-e)^2
-      RowSums m{0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) m.top = max_abs_nan(m.top, RowType<T>::get(v[k].e[i]));
-      m = reduce<G, false, false>(m);
-      const int e = odd ? ilogbf(m.top) : 0;
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float q = ldexpf(RowType<T>::get(v[k].e[i]), -e);
-          m.ss = fmaf(q, q, m.ss);
-        }
-      m = reduce<G, false, true>(m);
-      if (odd) {
-        const double mean = ldexp((double)m.ss * (double)P.inv_n, 2 * e) + (double)P.eps;
-        scale = (float)((double)r.top / 127.0 / sqrt(mean));
-      }
+      const float s = wide_range_scale<T, E, G>(x, d, r.top, P.inv_n, P.eps, odd);
+      if (odd) scale = s;
     }
   }
   if (dst < 0) return;  // nothing below needs the other lanes
@@ -254,54 +275,35 @@ __global__ void __launch_bounds__(quantize_threads(G)) k_quantize_rows(QuantizeP
   if (lane == 0) P.scales[dst] = scale;
 
   int8_t* out = P.codes + dst * P.code_stride;
-  // tiny rows are brought into range by a power of two, so 127 / top stays finite
-  const float pre = r.top < 1e-18f ? 1.2089258196146292e24f : 1.f;  // 2^80
-  const float inv = bad || r.top == 0.f ? 0.f : 127.f / (r.top * pre);
+  // rows so small that 127 / top may overflow take the 64-bit quotient throughout
+  const bool tiny = r.top < 1e-18f;
+  const float inv = bad || tiny ? 0.f : 127.f / r.top;
+  const float hi = fmaf(inv, 4.76837158203125e-07f, inv), lo = fmaf(inv, -4.76837158203125e-07f, inv);
+  uint32_t unsure = tiny && r.top > 0.f ? FULL_MASK : 0u;  // vectors to be done again
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = (k * G + lane) * V;
-    uint32_t n[V];
-    float off = 0.f;
+    const int c = (k * G + lane) * E;
+    if (c >= d) break;
+    float w[FULL ? E : 1];
+    if constexpr (FULL) load_weights<T, E>(P, c, d, w);
+    uint32_t n[E], differ = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float t;
-      if constexpr (FULL) t = u[k][i];
-      else t = RowType<T>::get(v[k].e[i]);
-      if (pre != 1.f) t *= pre;
-      const float big = fmaf(t, inv, ROUNDER);
-      off = fmaxf(off, fabsf(fmaf(t, inv, ROUNDER - big)));
-      n[i] = __float_as_uint(big);
+    for (int i = 0; i < E; ++i) {
+      float t = RowType<T>::get(v[k].e[i]);
+      if constexpr (FULL) t *= w[i];
+      n[i] = __float_as_uint(fmaf(t, hi, ROUNDER));
+      differ |= n[i] ^ __float_as_uint(fmaf(t, lo, ROUNDER));
     }
-    if (off > NEAR_HALF) {
-      const double a = (double)r.top + (double)r.low;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float w = 1.f;
-        if constexpr (FULL) {
-          if (P.w && c + i < d)
-            w = P.w_f32 ? __ldg(reinterpret_cast<const float*>(P.w) + c + i)
-                        : RowType<T>::get(reinterpret_cast<const T*>(P.w)[c + i]);
-        }
-        n[i] = (uint32_t)code_near_half(RowType<T>::get(v[k].e[i]), w, a);
+    if (differ) unsure |= 1u << k;
+    store_codes<E>(out, c, n, bad);
+  }
+  if (unsure && !bad) {
+    const double a = (double)r.top + (double)r.low;
+    for (int k = 0; k < NV; ++k)
+      if (unsure >> k & 1u) {
+        const int c = (k * G + lane) * E;
+        if (c < d) exact_codes<T>(P, x, out, c, E, a);
       }
-    }
-    if (bad) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) n[i] = 0;
-    }
-    uint32_t q[V / 4];
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i)
-      q[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040),
-                         0x5410);
-    if (P.wide_out && c + V <= d) {
-      if constexpr (V == 4) *reinterpret_cast<uint32_t*>(out + c) = q[0];
-      else *reinterpret_cast<uint2*>(out + c) = make_uint2(q[0], q[1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (c + i < d) out[c + i] = (int8_t)(q[i / 4] >> (8 * (i % 4)));
-    }
   }
 }
 
@@ -312,101 +314,125 @@ struct ReadParams {
   const void* ids;  // nullptr: row i
   void* out;
   int64_t n, rows, code_stride, out_stride;
-  int d, id64, wide_in, wide_out;
+  int d, id64;
 };
 
-// A warp reads R rows together (their loads are in flight at once), 16 bytes of
-// output a lane, row and step.  An id below 0 is an empty place (zeros), one past
-// the store a mistake (NaN).
-template <typename T, int R>
-__global__ void __launch_bounds__(256) k_dequantize_rows(ReadParams P) {
-  constexpr int V = RowType<T>::V;
-  const int lane = threadIdx.x & 31;
-  const int64_t i0 = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) / 32 * R;
-  if (i0 >= P.n) return;
-  bool known[R];
-  float scale[R];
-  const int8_t* in[R];
+// G lanes a row and E elements a step; NV steps' codes are in flight at once.  An
+// id below 0 is an empty place (zeros), one past the store a mistake (NaN).
+template <typename T, int E, int G, int NV>
+__global__ void __launch_bounds__(256) k_dequantize_rows(const __grid_constant__ ReadParams P) {
+  const int lane = threadIdx.x % G;
+  const int64_t i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  if (i >= P.n) return;
+  const int64_t id = P.ids ? slot_at(P.ids, P.id64, i) : i;
+  const bool known = id >= 0 && id < P.rows;
+  const float scale = known ? __ldg(P.scales + id) : id < 0 ? 0.f : __uint_as_float(0x7fffffffu);
+  const int8_t* in = P.codes + (known ? id : 0) * P.code_stride;
+  T* out = reinterpret_cast<T*>(P.out) + i * P.out_stride;
+  const int d = P.d, dk = known ? P.d : 0;
+  for (int c0 = lane * E; c0 < d; c0 += NV * G * E) {
+    uint32_t w[NV][(E + 3) / 4];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    int64_t id = -1;
-    if (i0 + r < P.n) id = P.ids ? slot_at(P.ids, P.id64, i0 + r) : i0 + r;
-    known[r] = id >= 0 && id < P.rows;
-    scale[r] = known[r] ? __ldg(P.scales + id) : id < 0 ? 0.f : __uint_as_float(0x7fffffffu);
-    in[r] = P.codes + (known[r] ? id : 0) * P.code_stride;
-  }
-  for (int c = lane * V; c < P.d; c += 32 * V) {
-    uint32_t w[R][V / 4];
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * G * E;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int k = 0; k < V / 4; ++k) w[r][k] = 0;
-      if (!known[r]) continue;
-      if (P.wide_in && c + V <= P.d) {
-        if constexpr (V == 4) {
-          w[r][0] = __ldg(reinterpret_cast<const uint32_t*>(in[r] + c));
+      for (int j = 0; j < (E + 3) / 4; ++j) w[k][j] = 0;
+      if (c < dk) {
+        if constexpr (E == 1) {
+          w[k][0] = (uint32_t)(uint8_t)__ldg(in + c);
+        } else if constexpr (E == 4) {
+          w[k][0] = __ldg(reinterpret_cast<const uint32_t*>(in + c));
         } else {
-          const uint2 b = __ldg(reinterpret_cast<const uint2*>(in[r] + c));
-          w[r][0] = b.x;
-          w[r][1] = b.y;
+          const uint2 b = __ldg(reinterpret_cast<const uint2*>(in + c));
+          w[k][0] = b.x;
+          w[k][1] = b.y;
         }
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (c + k < P.d) w[r][k / 4] |= (uint32_t)(uint8_t)__ldg(in[r] + c + k) << (8 * (k % 4));
       }
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (i0 + r >= P.n) break;
-      Vec<T> v;
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * G * E;
+      if (c >= d) break;
+      Vec<T, E> v;
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
+      for (int j = 0; j < E; ++j) {
         // code + 128 in the low byte of 2^23, less 2^23 + 128: the code as a float
-        const uint32_t biased = w[r][k / 4] ^ 0x80808080u;
-        const float code = __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7540 | (k % 4))) - 8388736.f;
-        v.e[k] = RowType<T>::put(code * scale[r]);  // the value's one rounding
+        const float code =
+            __uint_as_float(__byte_perm(w[k][j / 4] ^ 0x80808080u, 0x4b000000u, 0x7540 | (j % 4))) - 8388736.f;
+        v.e[j] = RowType<T>::put(code * scale);  // the value's one rounding
       }
-      store_vec(reinterpret_cast<T*>(P.out) + (i0 + r) * P.out_stride, c, P.d, P.wide_out, v);
+      v.store(out, c, d);
     }
   }
 }
 
 // ---------------------------------------------------------------- host side
-template <typename T, int G, int NV, bool FULL>
+// Lanes a row and vectors a lane.  Many rows: the fewest lanes (8, 16, 32) that
+// hold the row in at most 8 vectors each.  Few rows (less than four warps an SM
+// with a warp a row) are latency: a warp each, from 4 vectors a lane on a block
+// of 128 or 512.  Rows that are not whole 16-byte vectors on 16 bytes go element
+// by element, neighbouring lanes on neighbouring elements.
+constexpr int64_t FEW_ROWS = 148 * 4;
+
+template <typename T, int E, int G, int NV, bool FULL>
 static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
-  constexpr int threads = quantize_threads(G), rows = threads / G;
-  k_quantize_rows<T, G, NV, FULL><<<(unsigned)((P.n + rows - 1) / rows), threads, 0, st>>>(P);
+  constexpr int threads = row_threads(G), rows = threads / G;
+  k_quantize_rows<T, E, G, NV, FULL><<<(unsigned)((P.n + rows - 1) / rows), threads, 0, st>>>(P);
 }
-template <typename T, int G, bool FULL>
-static void quantize_nv(const QuantizeParams& P, int vectors, cudaStream_t st) {
-  const int nv = (vectors + G - 1) / G;
-  if (nv <= 1) launch_quantize<T, G, 1, FULL>(P, st);
-  else if (nv <= 2) launch_quantize<T, G, 2, FULL>(P, st);
-  else if (nv <= 3) launch_quantize<T, G, 3, FULL>(P, st);
-  else if (G < 512 || RowType<T>::V == 8 || nv <= 4) launch_quantize<T, G, 4, FULL>(P, st);
-  else if constexpr (G == 512 && RowType<T>::V == 4) launch_quantize<T, G, 8, FULL>(P, st);
-}
-// Threads a row: 8 lanes while they hold the row in at most 4 vectors each, then
-// a warp, a block of 128 and a block of 512 (up to 8 vectors: 16,384 fp32 values).
 template <typename T, bool FULL>
-static void quantize(const QuantizeParams& P, cudaStream_t st) {
-  const int vectors = (P.d + RowType<T>::V - 1) / RowType<T>::V;
-  if (vectors <= 8 * 4) quantize_nv<T, 8, FULL>(P, vectors, st);
-  else if (vectors <= 32 * 4) quantize_nv<T, 32, FULL>(P, vectors, st);
-  else if (vectors <= 128 * 4) quantize_nv<T, 128, FULL>(P, vectors, st);
-  else quantize_nv<T, 512, FULL>(P, vectors, st);
+static void quantize(const QuantizeParams& P, bool wide, cudaStream_t st) {
+  constexpr int V = RowType<T>::V;
+  if (!wide) {
+    if (P.d <= 128) launch_quantize<T, 1, 32, 4, FULL>(P, st);
+    else if (P.d <= 512) launch_quantize<T, 1, 32, 16, FULL>(P, st);
+    else if (P.d <= 1024) launch_quantize<T, 1, 32, 32, FULL>(P, st);
+    else if (P.d <= 4096) launch_quantize<T, 1, 128, 32, FULL>(P, st);
+    else launch_quantize<T, 1, 512, 32, FULL>(P, st);
+    return;
+  }
+  const int vectors = P.d / V;
+  if (P.n <= FEW_ROWS && vectors > 8) {
+    if (vectors <= 32) launch_quantize<T, V, 32, 1, FULL>(P, st);
+    else if (vectors <= 64) launch_quantize<T, V, 32, 2, FULL>(P, st);
+    else if (vectors <= 128) launch_quantize<T, V, 32, 4, FULL>(P, st);
+    else if (vectors <= 512) launch_quantize<T, V, 128, 4, FULL>(P, st);
+    else if (vectors <= 2048) launch_quantize<T, V, 512, 4, FULL>(P, st);
+    else if constexpr (V == 4) launch_quantize<T, V, 512, 8, FULL>(P, st);
+  } else if (vectors <= 8) launch_quantize<T, V, 8, 1, FULL>(P, st);
+  else if (vectors <= 16) launch_quantize<T, V, 8, 2, FULL>(P, st);
+  else if (vectors <= 32) launch_quantize<T, V, 8, 4, FULL>(P, st);
+  else if (vectors <= 48) launch_quantize<T, V, 8, 6, FULL>(P, st);
+  else if (vectors <= 64) launch_quantize<T, V, 8, 8, FULL>(P, st);
+  else if (vectors <= 96) launch_quantize<T, V, 16, 6, FULL>(P, st);
+  else if (vectors <= 128) launch_quantize<T, V, 16, 8, FULL>(P, st);
+  else if (vectors <= 192) launch_quantize<T, V, 32, 6, FULL>(P, st);
+  else if (vectors <= 256) launch_quantize<T, V, 32, 8, FULL>(P, st);
+  else if (vectors <= 512) launch_quantize<T, V, 128, 4, FULL>(P, st);
+  else if (vectors <= 1024) launch_quantize<T, V, 128, 8, FULL>(P, st);
+  else if (vectors <= 2048) launch_quantize<T, V, 512, 4, FULL>(P, st);
+  else if constexpr (V == 4) launch_quantize<T, V, 512, 8, FULL>(P, st);
 }
 
-static void dequantize(const ReadParams& P, int dtype, cudaStream_t st) {
-  const bool many = P.n >= 148 * 32;
-  const unsigned blocks = (unsigned)(many ? (P.n + 31) / 32 : (P.n + 7) / 8);
-  if (dtype == CIRCUIT_F32) many ? k_dequantize_rows<float, 4><<<blocks, 256, 0, st>>>(P)
-                                 : k_dequantize_rows<float, 1><<<blocks, 256, 0, st>>>(P);
-  else if (dtype == CIRCUIT_F16) many ? k_dequantize_rows<__half, 4><<<blocks, 256, 0, st>>>(P)
-                                      : k_dequantize_rows<__half, 1><<<blocks, 256, 0, st>>>(P);
-  else many ? k_dequantize_rows<__nv_bfloat16, 4><<<blocks, 256, 0, st>>>(P)
-            : k_dequantize_rows<__nv_bfloat16, 1><<<blocks, 256, 0, st>>>(P);
+template <typename T, int E, int G, int NV>
+static void launch_read(const ReadParams& P, cudaStream_t st) {
+  constexpr int rows = 256 / G;
+  k_dequantize_rows<T, E, G, NV><<<(unsigned)((P.n + rows - 1) / rows), 256, 0, st>>>(P);
+}
+template <typename T>
+static void dequantize(const ReadParams& P, bool wide, cudaStream_t st) {
+  constexpr int V = RowType<T>::V;
+  const int vectors = P.d / V;
+  if (!wide) launch_read<T, 1, 32, 8>(P, st);
+  else if (vectors <= 8) launch_read<T, V, 8, 1>(P, st);
+  else if (P.n <= FEW_ROWS) launch_read<T, V, 32, 4>(P, st);
+  else if (vectors <= 16) launch_read<T, V, 8, 2>(P, st);
+  else if (vectors <= 32) launch_read<T, V, 8, 4>(P, st);
+  else if (vectors <= 48) launch_read<T, V, 8, 6>(P, st);
+  else if (vectors <= 64) launch_read<T, V, 8, 8>(P, st);
+  else if (vectors <= 96) launch_read<T, V, 16, 6>(P, st);
+  else if (vectors <= 128) launch_read<T, V, 16, 8>(P, st);
+  else if (vectors <= 192) launch_read<T, V, 32, 6>(P, st);
+  else launch_read<T, V, 32, 8>(P, st);
 }
 
 }  // namespace i8
@@ -462,10 +488,11 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
   P.inv_n = norm == CIRCUIT_NORM_RMS ? 1.f / (float)dim : 1.f;
   P.eps = eps;
   P.slot64 = slot_bytes == 8;
-  // one access a vector where the rows allow it
-  P.wide_in = (on16(rows, row_stride * e) ? 1 : 0) | (residual && on16(residual, residual_stride * e) ? 2 : 0) |
-              (residual && on16(summed, summed_stride * e) ? 4 : 0) | (weight && on16(weight, 0) ? 8 : 0);
-  P.wide_out = (((uintptr_t)codes | (uintptr_t)code_stride) & 7) == 0;
+  // whole 16-byte vectors, each one access
+  const int vec = 16 / e;
+  const bool wide = dim % vec == 0 && on16(rows, row_stride * e) &&
+                    (!residual || (on16(residual, residual_stride * e) && on16(summed, summed_stride * e))) &&
+                    on16(weight, 0) && ((uintptr_t)codes | (uintptr_t)code_stride) % vec == 0;
   cudaStream_t st = (cudaStream_t)stream;
   // Equal slots: each row of a short write looks through the later ones; a long
   // write claims its slots first, the claims standing in the scales.
@@ -476,9 +503,9 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
     k_claim_slots<<<blocks, 256, 0, st>>>(slots, P.slot64, n, capacity, scales);
   }
   const bool full = norm != CIRCUIT_NORM_NONE;
-  if (dtype == CIRCUIT_F32) full ? quantize<float, true>(P, st) : quantize<float, false>(P, st);
-  else if (dtype == CIRCUIT_F16) full ? quantize<__half, true>(P, st) : quantize<__half, false>(P, st);
-  else full ? quantize<__nv_bfloat16, true>(P, st) : quantize<__nv_bfloat16, false>(P, st);
+  if (dtype == CIRCUIT_F32) full ? quantize<float, true>(P, wide, st) : quantize<float, false>(P, wide, st);
+  else if (dtype == CIRCUIT_F16) full ? quantize<__half, true>(P, wide, st) : quantize<__half, false>(P, wide, st);
+  else full ? quantize<__nv_bfloat16, true>(P, wide, st) : quantize<__nv_bfloat16, false>(P, wide, st);
   return check(cudaGetLastError(), "quantize_rows launch");
 }
 
@@ -496,10 +523,13 @@ int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const f
   if (code_stride < dim || out_stride < dim) return bad("dequantize_rows: a row stride is smaller than dim");
   if ((uintptr_t)out % e || (uintptr_t)scales % 4 || (ids && (uintptr_t)ids % id_bytes))
     return bad("dequantize_rows: a pointer is not aligned to its type");
-  ReadParams P{codes, scales, ids, out, n, rows, code_stride, out_stride, dim, id_bytes == 8,
-               (((uintptr_t)codes | (uintptr_t)code_stride) & 7) == 0, on16(out, out_stride * e)};
+  const ReadParams P{codes, scales, ids, out, n, rows, code_stride, out_stride, dim, id_bytes == 8};
+  const int vec = 16 / e;
+  const bool wide = dim % vec == 0 && on16(out, out_stride * e) && ((uintptr_t)codes | (uintptr_t)code_stride) % vec == 0;
   cudaStream_t st = (cudaStream_t)stream;
-  dequantize(P, dtype, st);
+  if (dtype == CIRCUIT_F32) dequantize<float>(P, wide, st);
+  else if (dtype == CIRCUIT_F16) dequantize<__half>(P, wide, st);
+  else dequantize<__nv_bfloat16>(P, wide, st);
   return check(cudaGetLastError(), "dequantize_rows launch");
 }
 

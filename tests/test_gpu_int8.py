@@ -43,13 +43,14 @@ def _check_plain(x, codes, scales):
     assert torch.equal(scales, (a / 127).float())
 
 
-DIMS = [1, 2, 7, 16, 31, 33, 128, 384, 385, 511, 512, 513, 1000, 1024, 1025, 2048, 2049, 4096, 4100, 8191, 8192, 16384]
+DIMS = [1, 2, 7, 16, 31, 33, 64, 128, 136, 200, 256, 384, 385, 511, 512, 513, 640, 768, 1000, 1024, 1025, 1536, 2048, 2049,
+        4096, 4100, 8191, 8192, 16384]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", DIMS)
 def test_quantize_dims(d, dtype):
-    for n in (1, 5, 67):
+    for n in (1, 5, 67, 701):
         x = _rows(n, d, dtype, seed=d + n)
         codes, scales = quantize_rows(x)
         assert codes.shape == (n, d) and codes.dtype == torch.int8 and scales.dtype == torch.float32
@@ -90,8 +91,9 @@ def test_quantize_next_to_halves():
 def test_quantize_extreme_magnitudes(scale):
     x = _rows(6, 260, torch.float32, seed=1)
     x = (x.double() * scale).float()
-    codes, scales = quantize_rows(x)
-    _check_plain(x, codes, scales)
+    for y in (x, x[:, 1:], x.repeat(120, 1)):
+        codes, scales = quantize_rows(y)
+        _check_plain(y, codes, scales)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -134,7 +136,7 @@ def _check_norm(x, r, w, eps, got, unit=False):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", DIMS)
 def test_norm_dims(d, dtype):
-    for n in (1, 37):
+    for n in (1, 37, 613):
         x, r = _rows(n, d, dtype, seed=d), _rows(n, d, dtype, seed=d + 1, scale=0.3)
         w = (1 + 0.2 * _rows(1, d, torch.float32, seed=d + 2)[0])
         for rr, ww in ((r, w.to(dtype)), (r, w), (None, w), (r, None), (None, None)):
@@ -155,8 +157,10 @@ def test_norm_strides(dtype):
 @pytest.mark.parametrize("d", [384, 6000])
 def test_norm_extreme_magnitudes(scale, d):
     x = (_rows(5, d, torch.float32, seed=7).double() * scale).float()
-    _check_norm(x, None, None, 0.0, rms_norm_quantize(x, eps=0.0))
-    _check_norm(x, None, None, 1e-6, rms_norm_quantize(x, eps=1e-6))
+    mixed = torch.cat([x, _rows(5, d, torch.float32, seed=8)]).repeat(80, 1)  # rows in and out of range in one warp
+    for y in (x, x[:, 1:], mixed):
+        _check_norm(y, None, None, 0.0, rms_norm_quantize(y, eps=0.0))
+        _check_norm(y, None, None, 1e-6, rms_norm_quantize(y, eps=1e-6))
 
 
 def test_norm_sum_overflows_its_type():
