@@ -27,12 +27,11 @@ MOST_ROW_BYTES = 800e6  # of the largest store that a product reads
 
 
 def _ops():
-    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "circuit-rag_b200")
-    if here not in sys.path:
-        sys.path.insert(0, here)
-    import circuit_rag
-
-    return circuit_rag
+    package = sys.modules.get("circuit_rag")
+    if package is None:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "circuit-rag_b200"))
+        import circuit_rag as package
+    return package
 
 
 def listed():
