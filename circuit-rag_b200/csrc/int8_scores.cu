@@ -21,9 +21,8 @@ struct ScoresParams {
   int pairs;  // two neighbouring 16-bit results of a row of `out` may be stored as one
 };
 
-template <typename T>
-__device__ __forceinline__ T scored(int acc, float sq, float sr, float bias) {
-  return RowType<T>::put(fmaf((float)acc * sq, sr, bias));
+__device__ __forceinline__ float result(int acc, float sq, float sr, float bias) {
+  return fmaf((float)acc * sq, sr, bias);
 }
 
 // Eight lanes a row, each with 16 codes a step, NQ queries in shared memory
@@ -62,7 +61,8 @@ __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
       for (int o = 4; o > 0; o >>= 1) acc[q] += __shfl_xor_sync(FULL_MASK, acc[q], o);
       if (live && sub == (q & 7) && q0 + q < P.nq)
         reinterpret_cast<T*>(P.out)[(q0 + q) * P.out_stride + row] =
-            scored<T>(acc[q], __ldg(P.q_scales + q0 + q), __ldg(P.scales + row), P.bias ? __ldg(P.bias + row) : 0.f);
+            RowType<T>::put(result(acc[q], __ldg(P.q_scales + q0 + q), __ldg(P.scales + row),
+                                   P.bias ? __ldg(P.bias + row) : 0.f));
     }
   }
 }
@@ -77,8 +77,30 @@ __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
 // and a column a query: each warp store writes 32 consecutive results of one
 // query's row of `out`, without a transposition.
 constexpr int MMA_ROWS = 128;
-constexpr int epilogue_warps(int BN) { return BN >= 64 ? 8 : 4; }          // then a TMA and an MMA warp
+// Epilogue warps: a result is an integer conversion (a quarter-rate instruction: 2,048
+// clocks for a 128 x 256 tile), two products, an address and a store, so a tile's
+// results take many warps to keep pace; then a TMA and an MMA warp.
+constexpr int epilogue_warps(int BN) { return BN >= 256 ? 16 : BN >= 64 ? 8 : 4; }
 constexpr int mma_threads(int BN) { return (epilogue_warps(BN) + 2) * 32; }
+
+// Units first, first + step, ... as (row tile, query tile), query tiles fastest,
+// without a division a unit.
+struct Units {
+  int64_t u, step, rt, step_rt;
+  int qt, step_qt, q_tiles;
+  __device__ __forceinline__ Units(int64_t first, int64_t by, int tiles)
+      : u(first), step(by), rt(first / tiles), step_rt(by / tiles), qt((int)(first % tiles)), step_qt((int)(by % tiles)),
+        q_tiles(tiles) {}
+  __device__ __forceinline__ void next() {
+    u += step;
+    rt += step_rt;
+    qt += step_qt;
+    if (qt >= q_tiles) {
+      qt -= q_tiles;
+      ++rt;
+    }
+  }
+};
 constexpr int RING_BYTES = 192 * 1024;
 constexpr int chunk_bytes(int BN) { return (MMA_ROWS + BN) * 128; }
 constexpr int ring_stages(int BN) { return RING_BYTES / chunk_bytes(BN); }
@@ -86,49 +108,114 @@ constexpr int ring_stages(int BN) { return RING_BYTES / chunk_bytes(BN); }
 // Bits of the waits that gave up, kept until circuit_op_int8_status reads them.
 __device__ int g_error;
 
-// One result a lane (a row) and column (a query), COLS columns from tmem: in full
-// tiles every lane and column counts.
-template <int W>
-__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[W]) {
-  if constexpr (W == 32) tc::ld_32x32b_x32(taddr, v);
-  else tc::ld_32x32b_x16(taddr, v);
+// Two results as the 16-bit values of one word.
+__device__ __forceinline__ uint32_t two(__half, float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return reinterpret_cast<const uint32_t&>(h);
 }
-// W results of a lane, W queries apart by ld.  `left` queries and live rows count.
-// 16-bit results of full tiles go out as pairs of rows: neighbouring lanes swap
-// one of every two columns, so that a warp store fills 64 bytes of two queries.
+__device__ __forceinline__ uint32_t two(__nv_bfloat16, float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return reinterpret_cast<const uint32_t&>(h);
+}
+
+// W results of a lane's row, for queries `ld` bytes apart from `out` on.  `left` of
+// them and live rows count.  16-bit results of full tiles go out as pairs of rows:
+// neighbouring lanes swap one of every two columns, so that a warp store fills 64
+// bytes of two queries.
 template <typename T, int W>
-__device__ __forceinline__ void store_columns(T* out, int64_t ld, const uint32_t (&v)[W], const float* sq, float sr,
-                                              float bias, bool live, int64_t left, bool pairs) {
+__device__ __forceinline__ void store_columns(char* out, uint32_t ld, int64_t ld64, const uint32_t (&v)[W],
+                                              const float* sq, float sr, float bias, bool live, int64_t left,
+                                              bool pairs) {
   float s[W];
 #pragma unroll
   for (int i = 0; i < W; i += 4) *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(sq + i);
   if constexpr (sizeof(T) == 2) {
     if (pairs && left >= W) {
       const bool odd = threadIdx.x & 1;
-      T* o = out + (odd ? ld - 1 : 0);
+      const uint32_t pick = odd ? 0x3276u : 0x5410u;
+      char* o = out + (odd ? (int64_t)ld - 2 : 0);
 #pragma unroll
       for (int i = 0; i < W; i += 2) {
-        const T a = scored<T>((int)v[i], s[i], sr, bias), b = scored<T>((int)v[i + 1], s[i + 1], sr, bias);
-        const uint32_t ua = reinterpret_cast<const uint16_t&>(a), ub = reinterpret_cast<const uint16_t&>(b);
-        const uint32_t got = __shfl_xor_sync(FULL_MASK, odd ? ua : ub, 1);
-        *reinterpret_cast<uint32_t*>(o) = odd ? got | ub << 16 : ua | got << 16;
-        o += 2 * ld;
+        const uint32_t mine = two(T{}, result((int)v[i], s[i], sr, bias), result((int)v[i + 1], s[i + 1], sr, bias));
+        // even lanes keep column i of both rows, odd lanes column i + 1
+        const uint32_t other = __shfl_xor_sync(FULL_MASK, mine, 1);
+        *reinterpret_cast<uint32_t*>(o + (uint64_t)ld * (uint32_t)i) = __byte_perm(mine, other, pick);
       }
       return;
     }
   }
   if (!live) return;
-  if (left >= W) {
+  if (left >= W && ld) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      *out = scored<T>((int)v[i], s[i], sr, bias);
-      out += ld;
-    }
+    for (int i = 0; i < W; ++i)
+      *reinterpret_cast<T*>(out + (uint64_t)ld * (uint32_t)i) = RowType<T>::put(result((int)v[i], s[i], sr, bias));
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i)
-      if (i < (int)left) out[i * ld] = scored<T>((int)v[i], s[i], sr, bias);
+      if (i < left) *reinterpret_cast<T*>(out + ld64 * i) = RowType<T>::put(result((int)v[i], s[i], sr, bias));
   }
+}
+
+// An epilogue warp's loop over its units: 32 rows of the tile (its TMEM lanes) from
+// row_off on, COLS columns.  The next unit's scales and the next 16 columns are on
+// their way while the present ones are stored.  Once a wait has given up, the
+// results that it would have brought are NaN.
+template <typename T, int COLS, typename Release>
+__device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, int BN, float* sq, Units un,
+                                         int64_t units, int tile_rows, int row_off, uint64_t* acc_full,
+                                         Release release) {
+  constexpr int W = 16, N = COLS / W, SQ = (COLS + 31) / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, part = warp >> 2;
+  const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(part * COLS);
+  const int64_t ld64 = P.out_stride * (int64_t)sizeof(T);
+  const uint32_t ld = ld64 < (1ll << 32) ? (uint32_t)ld64 : 0u;
+  float sr = 0.f, bias = 0.f, sqv[SQ];
+  int64_t row0 = 0, q0 = 0;
+  auto fetch = [&]() {  // of unit un
+    row0 = un.rt * tile_rows + row_off + 32 * quarter;
+    q0 = (int64_t)un.qt * BN + part * COLS;
+    const bool live = row0 + lane < P.n;
+    sr = live ? __ldg(P.scales + row0 + lane) : 0.f;
+    bias = live && P.bias ? __ldg(P.bias + row0 + lane) : 0.f;
+#pragma unroll
+    for (int i = 0; i < SQ; ++i)
+      sqv[i] = 32 * i + lane < COLS && q0 + 32 * i + lane < P.nq ? __ldg(P.q_scales + q0 + 32 * i + lane) : 0.f;
+  };
+  if (un.u < units) fetch();
+  bool ok = true;
+  for (int it = 0; un.u < units; ++it) {
+    const int b = it & 1;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < SQ; ++i)
+      if (32 * i + lane < COLS) sq[32 * i + lane] = sqv[i];
+    __syncwarp();
+    const int64_t row = row0 + lane, left = P.nq - q0;
+    const bool pairs = P.pairs && ld && row0 + 32 <= P.n;
+    char* out = reinterpret_cast<char*>(P.out) + q0 * ld64 + row * (int64_t)sizeof(T);
+    float s = sr;
+    const float bb = bias;
+    un.next();
+    if (un.u < units) fetch();
+    ok = ok && __all_sync(FULL_MASK, mbar_wait(&acc_full[b], (uint32_t)(it / 2) & 1u, &g_error, ERR_TIMEOUT_FULL));
+    if (!ok) s = __uint_as_float(0x7fffffffu);
+    tc::fence_after();
+    uint32_t v[2][W];
+    tc::ld_32x32b_x16(taddr + (uint32_t)(b * BN), v[0]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      tc::wait_ld();
+      if (i + 1 < N) {
+        tc::ld_32x32b_x16(taddr + (uint32_t)(b * BN + (i + 1) * W), v[(i + 1) & 1]);
+      } else {
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) release(b);
+      }
+      store_columns<T, W>(out + i * W * ld64, ld, ld64, v[i & 1], sq + i * W, s, bb, row < P.n, left - i * W, pairs);
+    }
+  }
+  return ok;
 }
 
 template <typename T, int BN>
@@ -136,7 +223,6 @@ __global__ void __launch_bounds__(mma_threads(BN), 1)
     k_scores_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
                  int q_tiles, int64_t units) {
   constexpr int S = ring_stages(BN), STAGE = chunk_bytes(BN), EW = epilogue_warps(BN), COLS = BN / (EW / 4);
-  constexpr int W = COLS < 32 ? COLS : 32;  // columns of one TMEM load
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -170,9 +256,8 @@ __global__ void __launch_bounds__(mma_threads(BN), 1)
       int64_t filled = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const int64_t rt = u / q_tiles;
-        const int row0 = (int)(rt * MMA_ROWS), q0 = (int)(u - rt * q_tiles) * BN;
+      for (Units un(blockIdx.x, gridDim.x, q_tiles); un.u < units && ok; un.next()) {
+        const int row0 = (int)(un.rt * MMA_ROWS), q0 = un.qt * BN;
         for (int j = 0; j < chunks; ++j, ++filled) {
           if (filled >= S && !mbar_wait(&empty[s], ph ^ 1u, &g_error, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
           mbar_arrive_expect_tx(&full[s], STAGE);  // out-of-range rows and columns arrive as zeros
@@ -223,50 +308,142 @@ __global__ void __launch_bounds__(mma_threads(BN), 1)
     }
     if (!ok && lane == 0) s_failed = 1;
   } else {
-    const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
-    float* sq = s_sq[warp];
-    int64_t loaded = -1;
-    int it = 0;
-    bool ok = true;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x, ++it) {
-      const int b = it & 1;
-      const int64_t rt = u / q_tiles, row = rt * MMA_ROWS + 32 * quarter + lane;
-      const int64_t q0 = (u - rt * q_tiles) * BN + half * COLS;
-      const bool live = row < P.n;
-      float sr = live ? __ldg(P.scales + row) : 0.f;
-      const float bias = live && P.bias ? __ldg(P.bias + row) : 0.f;
-      if (q0 != loaded) {
-        __syncwarp();
-        for (int i = lane; i < COLS; i += 32) sq[i] = q0 + i < P.nq ? __ldg(P.q_scales + q0 + i) : 0.f;
-        __syncwarp();
-        loaded = q0;
-      }
-      // once a wait has given up, the results that it would have brought are NaN
-      ok = ok && __all_sync(FULL_MASK, mbar_wait(&acc_full[b], (uint32_t)(it / 2) & 1u, &g_error, ERR_TIMEOUT_FULL));
-      if (!ok) sr = __uint_as_float(0x7fffffffu);
-      tc::fence_after();
-      const bool pairs = P.pairs && rt * MMA_ROWS + 32 * quarter + 32 <= P.n;
-      T* out = reinterpret_cast<T*>(P.out) + q0 * P.out_stride + row;
-#pragma unroll 1
-      for (int c = 0; c < COLS; c += W) {
-        uint32_t v[W];
-        load_columns<W>(tmem + lane_base + (uint32_t)(b * BN + half * COLS + c), v);
-        tc::wait_ld();
-        if (c + W == COLS) {
-          tc::fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[b]);
-        }
-        store_columns<T, W>(out + c * P.out_stride, P.out_stride, v, sq + c, sr, bias, live, P.nq - q0 - c, pairs);
-      }
-    }
+    const bool ok = epilogue<T, COLS>(P, tmem, BN, s_sq[warp], Units(blockIdx.x, gridDim.x, q_tiles), units, MMA_ROWS, 0,
+                                      acc_full, [&](int b) { mbar_arrive(&acc_empty[b]); });
     if (!ok && lane == 0) s_failed = 1;
   }
   tc::fence_before();
   __syncthreads();
   if (s_failed) grace_period();  // copies and MMAs of the failed waits end before the memory is freed
   if (warp == EW + 1) tc::tmem_dealloc(tmem, 2 * BN);
+}
+
+// The same for many queries with a CTA pair a unit of 256 rows x 256 queries: each
+// CTA loads 128 rows and 128 queries of a chunk (32 KB against the 48 KB of a
+// single CTA's 128 x 256 tile, and the operands' way from L2 is what bounds the
+// single CTA), the even CTA issues MMAs over both CTAs' shared memory, and each
+// CTA's TMEM holds its 128 rows against all 256 queries.
+constexpr int PAIR_BN = 256;
+constexpr int PAIR_STAGE = (MMA_ROWS + PAIR_BN / 2) * 128;
+constexpr int PAIR_STAGES = RING_BYTES / PAIR_STAGE;
+constexpr int PAIR_EW = epilogue_warps(PAIR_BN);
+
+template <typename T>
+__global__ void __launch_bounds__(mma_threads(PAIR_BN), 1)
+    k_scores_pair(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
+                  int q_tiles, int64_t units) {
+  constexpr int S = PAIR_STAGES, EW = PAIR_EW, COLS = PAIR_BN / (EW / 4);
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  // full and acc_empty are used in the even CTA only, empty and acc_full in both
+  __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ int s_failed;
+  __shared__ __align__(16) float s_sq[EW][COLS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = (P.d + 127) >> 7;
+  const uint32_t rank = tc::cluster_ctarank();
+  const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * EW);  // one lane of each epilogue warp of both CTAs
+    }
+    s_failed = 0;
+    tc::fence_mbar_init_cluster();
+    fence_mbar_init();
+  }
+  if (warp == EW + 1) tc::tmem_alloc_pair(&tmem_base, 2 * PAIR_BN);
+  tc::fence_before();
+  tc::cluster_sync();  // barriers and the pair's TMEM exist before any remote access
+  tc::fence_after();
+  const uint32_t tmem = tmem_base;
+  const uint32_t lead_full = tc::mapa_shared(smem_u32(&full[0]), 0);
+  const uint32_t lead_acc_empty = tc::mapa_shared(smem_u32(&acc_empty[0]), 0);
+
+  if (warp == EW) {
+    if (lane == 0) {
+      int s = 0;
+      int64_t filled = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (Units un(first, step, q_tiles); un.u < units && ok; un.next()) {
+        const int row0 = (int)(un.rt * 2 * MMA_ROWS + rank * MMA_ROWS);
+        const int q0 = un.qt * PAIR_BN + (int)rank * (PAIR_BN / 2);
+        for (int j = 0; j < chunks; ++j, ++filled) {
+          if (filled >= S && !mbar_wait(&empty[s], ph ^ 1u, &g_error, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * PAIR_STAGE);  // both CTAs' copies
+          unsigned char* dst = smem + s * PAIR_STAGE;
+          const uint32_t bar = lead_full + 8u * (uint32_t)s;
+          tc::tma_load_2d_pair(dst, &cmap, 128 * j, row0, bar);
+          tc::tma_load_2d_pair(dst + MMA_ROWS * 128, &qmap, 128 * j, q0, bar);
+          if (++s == S) { s = 0; ph ^= 1u; }
+        }
+      }
+      for (int64_t t = filled > S ? filled - S : 0; t < filled && ok; ++t)
+        ok = mbar_wait(&empty[t % S], (uint32_t)(t / S) & 1u, &g_error, ERR_TIMEOUT_EMPTY);
+      if (!ok) s_failed = 1;
+    }
+  } else if (warp == EW + 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc = tc::idesc_s8(2 * MMA_ROWS, PAIR_BN);
+      const uint32_t sbase = smem_u32(smem);
+      const uint64_t dA = tc::sdesc_k_sw128(sbase), dB = tc::sdesc_k_sw128(sbase + MMA_ROWS * 128);
+      const uint32_t empty0 = tc::mapa_shared(smem_u32(&empty[0]), 0), empty1 = tc::mapa_shared(smem_u32(&empty[0]), 1);
+      const uint32_t accf0 = tc::mapa_shared(smem_u32(&acc_full[0]), 0);
+      const uint32_t accf1 = tc::mapa_shared(smem_u32(&acc_full[0]), 1);
+      const int tail = (P.d - (chunks - 1) * 128 + 31) >> 5;
+      int s = 0, it = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int64_t u = first; u < units && ok; u += step, ++it) {
+        const int b = it & 1;
+        if (it >= 2 && !__all_sync(FULL_MASK, tc::mbar_wait_cluster(&acc_empty[b], (uint32_t)(it / 2 - 1) & 1u, &g_error,
+                                                                    ERR_TIMEOUT_EMPTY))) {
+          ok = false;
+          break;
+        }
+        tc::fence_after();
+        const uint32_t acc = tmem + (uint32_t)(b * PAIR_BN);
+        for (int j = 0; j < chunks; ++j) {
+          if (!__all_sync(FULL_MASK, mbar_wait(&full[s], ph, &g_error, ERR_TIMEOUT_FULL))) { ok = false; break; }
+          tc::fence_after();
+          if (tc::elect_one()) {
+            const uint64_t off = (uint64_t)((uint32_t)(s * PAIR_STAGE) >> 4);
+            const int steps = j + 1 < chunks ? 4 : tail;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (k < steps) tc::mma_s8_ss_pair(acc, dA + off + 2 * k, dB + off + 2 * k, idesc, (j | k) != 0 ? 1u : 0u);
+            tc::commit_pair(empty0 + 8u * (uint32_t)s);
+            tc::commit_pair(empty1 + 8u * (uint32_t)s);
+          }
+          __syncwarp();
+          if (++s == S) { s = 0; ph ^= 1u; }
+        }
+        if (ok && tc::elect_one()) {
+          tc::commit_pair(accf0 + 8u * (uint32_t)b);
+          tc::commit_pair(accf1 + 8u * (uint32_t)b);
+        }
+        __syncwarp();
+      }
+      if (!ok && lane == 0) s_failed = 1;
+    }
+  } else {
+    const bool ok = epilogue<T, COLS>(P, tmem, PAIR_BN, s_sq[warp], Units(first, step, q_tiles), units, 2 * MMA_ROWS,
+                                      (int)rank * MMA_ROWS, acc_full,
+                                      [&](int b) { tc::mbar_arrive_remote(lead_acc_empty + 8u * (uint32_t)b); });
+    if (!ok && lane == 0) s_failed = 1;
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (s_failed) grace_period();  // copies and MMAs of the failed waits end before the memory is freed
+  tc::cluster_sync();  // neither CTA leaves while the other may still arrive on its barriers
+  if (warp == EW + 1) tc::tmem_dealloc_pair(tmem, 2 * PAIR_BN);
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
@@ -327,6 +504,32 @@ static int launch_rows(const ScoresParams& P, cudaStream_t st) {
   return CIRCUIT_OK;
 }
 template <typename T>
+static int launch_pair(const ScoresParams& P, cudaStream_t st) {
+  CUtensorMap qmap, cmap;
+  if (!code_map(&qmap, P.q, P.nq, P.d, P.q_stride, PAIR_BN / 2) ||
+      !code_map(&cmap, P.codes, P.n, P.d, P.code_stride, MMA_ROWS))
+    return bad("int8_scores: cuTensorMapEncodeTiled refused the code rows");
+  constexpr int smem = PAIR_STAGES * PAIR_STAGE + 1024;
+  const int rc = check(cudaFuncSetAttribute(k_scores_pair<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                       "int8_scores shared memory");
+  if (rc) return rc;
+  const int q_tiles = (int)((P.nq + PAIR_BN - 1) / PAIR_BN);
+  const int64_t units = (P.n + 2 * MMA_ROWS - 1) / (2 * MMA_ROWS) * q_tiles, pairs = sm_count() / 2;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = 2;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(2 * (units < pairs ? units : pairs)));
+  cfg.blockDim = dim3(mma_threads(PAIR_BN));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  return check(cudaLaunchKernelEx(&cfg, k_scores_pair<T>, qmap, cmap, P, q_tiles, units), "int8_scores launch");
+}
+
+template <typename T>
 static int scores(const ScoresParams& P, cudaStream_t st) {
   // One or two queries on few bytes: the row kernel starts faster (5,183 x 384: 3.0 against 3.6 us, 4,096 x 2,048: 5.5
   // against 7.1); from 16 MB on the ring of bulk copies keeps more in flight (50,000 x 384: 5.8 and 5.9 us,
@@ -337,7 +540,8 @@ static int scores(const ScoresParams& P, cudaStream_t st) {
   if (P.nq <= 32) return launch_mma<T, 32>(P, st);
   if (P.nq <= 64) return launch_mma<T, 64>(P, st);
   if (P.nq <= 128) return launch_mma<T, 128>(P, st);
-  return launch_mma<T, 256>(P, st);
+  if (getenv("I8_SINGLE")) return launch_mma<T, 256>(P, st);
+  return launch_pair<T>(P, st);
 }
 
 }  // namespace i8
