@@ -121,7 +121,8 @@ __device__ __forceinline__ uint32_t two(__nv_bfloat16, float lo, float hi) {
 // W results of a lane's row, for queries `ld` bytes apart from `out` on.  `left` of
 // them and live rows count.  16-bit results of full tiles go out as pairs of rows:
 // neighbouring lanes swap one of every two columns, so that a warp store fills 64
-// bytes of two queries.
+// bytes of two queries.  Stores are marked as streaming, so that the results do not
+// push the rows out of L2 (256 x 400,000 x 384 fp32: 114 -> 109 us).
 template <typename T, int W>
 __device__ __forceinline__ void store_columns(char* out, uint32_t ld, int64_t ld64, const uint32_t (&v)[W],
                                               const float* sq, float sr, float bias, bool live, int64_t left,
@@ -139,7 +140,7 @@ __device__ __forceinline__ void store_columns(char* out, uint32_t ld, int64_t ld
         const uint32_t mine = two(T{}, result((int)v[i], s[i], sr, bias), result((int)v[i + 1], s[i + 1], sr, bias));
         // even lanes keep column i of both rows, odd lanes column i + 1
         const uint32_t other = __shfl_xor_sync(FULL_MASK, mine, 1);
-        *reinterpret_cast<uint32_t*>(o + (uint64_t)ld * (uint32_t)i) = __byte_perm(mine, other, pick);
+        __stcs(reinterpret_cast<uint32_t*>(o + (uint64_t)ld * (uint32_t)i), __byte_perm(mine, other, pick));
       }
       return;
     }
@@ -148,7 +149,7 @@ __device__ __forceinline__ void store_columns(char* out, uint32_t ld, int64_t ld
   if (left >= W && ld) {
 #pragma unroll
     for (int i = 0; i < W; ++i)
-      *reinterpret_cast<T*>(out + (uint64_t)ld * (uint32_t)i) = RowType<T>::put(result((int)v[i], s[i], sr, bias));
+      __stcs(reinterpret_cast<T*>(out + (uint64_t)ld * (uint32_t)i), RowType<T>::put(result((int)v[i], s[i], sr, bias)));
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i)
@@ -540,7 +541,6 @@ static int scores(const ScoresParams& P, cudaStream_t st) {
   if (P.nq <= 32) return launch_mma<T, 32>(P, st);
   if (P.nq <= 64) return launch_mma<T, 64>(P, st);
   if (P.nq <= 128) return launch_mma<T, 128>(P, st);
-  if (getenv("I8_SINGLE")) return launch_mma<T, 256>(P, st);
   return launch_pair<T>(P, st);
 }
 
