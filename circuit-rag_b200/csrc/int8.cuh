@@ -39,10 +39,11 @@ struct RowType<__nv_bfloat16> {
   __device__ static __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
 };
 
-// Maximum of magnitudes that keeps a NaN (fmaxf would drop it).
+// The larger magnitude, keeping a NaN (fmaxf would drop it); its sign is the product of
+// the operands' signs: the caller takes the magnitude at the end.
 __device__ __forceinline__ float max_abs_nan(float m, float x) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(x));
   return r;
 }
 
@@ -62,7 +63,7 @@ __device__ __forceinline__ void add_to(T (&a)[E], const T (&b)[E]) {
     }
   }
 }
-// top = max(top, |v|), a NaN stays.
+// |top| = max(|top|, |v|), a NaN stays.
 template <typename T, int E>
 __device__ __forceinline__ void raise_top(float& top, const T (&v)[E]) {
   if constexpr (sizeof(T) == 4 || E == 1) {

@@ -18,7 +18,8 @@ namespace i8 {
 
 // ---------------------------------------------------------------- helpers
 struct RowSums {
-  float top, low;  // max |u| as the unevaluated sum top + low (top: the rounded product); top NaN or inf: a bad row
+  float top, low;  // max |u| as the unevaluated sum top + low (top: the rounded product; its sign says nothing before
+                   // the reduction); top NaN or inf: a bad row
   float ss;        // sum of v^2
 };
 // (top, low) of two candidates: the larger real number; a NaN stays.
@@ -31,12 +32,13 @@ __device__ __forceinline__ void raise(float& top, float& low, float t, float l) 
 // Over the G threads of a row.
 template <int G, bool LOW, bool SS>
 __device__ __forceinline__ RowSums reduce(RowSums r) {
+  r.top = fabsf(r.top);
   constexpr int W = G < 32 ? G : 32;
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1) {
     const float t = __shfl_xor_sync(FULL_MASK, r.top, o);
     if constexpr (LOW) raise(r.top, r.low, t, __shfl_xor_sync(FULL_MASK, r.low, o));
-    else r.top = max_abs_nan(r.top, t);
+    else r.top = fabsf(max_abs_nan(r.top, t));
     if constexpr (SS) r.ss += __shfl_xor_sync(FULL_MASK, r.ss, o);
   }
   if constexpr (G > 32) {
@@ -48,7 +50,7 @@ __device__ __forceinline__ RowSums reduce(RowSums r) {
 #pragma unroll
     for (int w = 1; w < G / 32; ++w) {
       if constexpr (LOW) raise(r.top, r.low, part[w].top, part[w].low);
-      else r.top = max_abs_nan(r.top, part[w].top);
+      else r.top = fabsf(max_abs_nan(r.top, part[w].top));
       if constexpr (SS) r.ss += part[w].ss;
     }
   }
@@ -241,16 +243,22 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
     for (int k = 0; k < NV; ++k) {
       float w[E];
       load_weights<T, E>(P, (k * G + lane) * E, d, w);
+      float u[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float e = RowType<T>::get(v[k].e[i]), u = e * w[i];
+        const float e = RowType<T>::get(v[k].e[i]);
         r.ss = fmaf(e, e, r.ss);
-        if (P.inexact) {  // an fp32 factor: the FMA gives the product's rounding error
-          const float p = fabsf(u);
-          if (!(p < r.top)) raise(r.top, r.low, p, fmaf(fabsf(e), fabsf(w[i]), -p));
-        } else {  // 8- or 11-bit factors: their product is exact
-          r.top = max_abs_nan(r.top, u);
+        u[i] = e * w[i];
+      }
+      if (P.inexact) {  // an fp32 factor: the FMA gives the product's rounding error
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float p = fabsf(u[i]);
+          if (!(p < r.top)) raise(r.top, r.low, p, fmaf(fabsf(RowType<T>::get(v[k].e[i])), fabsf(w[i]), -p));
         }
+      } else {  // 8- or 11-bit factors: their product is exact
+#pragma unroll
+        for (int i = 0; i < E; ++i) r.top = max_abs_nan(r.top, u[i]);
       }
     }
     r = P.inexact ? reduce<G, true, true>(r) : reduce<G, false, true>(r);
