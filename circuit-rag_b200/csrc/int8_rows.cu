@@ -10,6 +10,7 @@
 // gives the correctly rounded code of the real quotient (see code_of), and only
 // the scale carries the rounding of the 32-bit sum of squares.
 #include <cfloat>
+#include <type_traits>
 
 #include "int8.cuh"
 
@@ -64,9 +65,23 @@ __device__ __forceinline__ RowSums reduce(RowSums r) {
 // both give the same integer it is the code, where not (within 127 2^-21 = 6e-5 of
 // a half: 0.006 % of the values) the quotient is taken in 64 bits, in which v * w
 // is exact.
+//
+// 16-bit values without a weight have m < 2^11 steps of their exponent, as has top
+// (ma): 127 v / top = 127 mv / (ma 2^k) is either a half, or 1 / (2 ma 2^k) >=
+// 2^-19 of its size away from one, more than hi's 10 * 2^-24.  A half needs 254 mv =
+// (2 n + 1) ma 2^k, so the prime 127 divides 2 n + 1 (which is then 127: v = top / 2,
+// a value that 16-bit rows often hold, and n = 63 goes to the even 64, as u * hi says)
+// or ma.  So hi alone gives the code unless 127 divides ma.
 constexpr float ROUNDER = 12582912.f;
 __device__ __forceinline__ int code_near_half(float v, float w, double a) {
   return (int)rint((double)v * (double)w * 127.0 / a);
+}
+
+// Whether 127 does not divide the significand of a 16-bit value's magnitude.
+template <typename T>
+__device__ __forceinline__ bool free_of_127(float top) {
+  constexpr int DROP = std::is_same<T, __half>::value ? 13 : 16;  // fp32 bits that the type does not have
+  return (((__float_as_uint(top) & 0x7fffffu) | 0x800000u) >> DROP) % 127u != 0u;
 }
 
 struct QuantizeParams {
@@ -105,7 +120,7 @@ __global__ void k_claim_slots(const void* slots, int slot64, int64_t n, int64_t 
   if (s >= 0 && s < capacity) atomicMax(reinterpret_cast<uint32_t*>(scales + s), claim_tag(i));
 }
 
-constexpr int row_threads(int G) { return G <= 32 ? 256 : G; }
+constexpr int row_threads(int G) { return G <= 32 ? 128 : G; }
 
 // The weights of elements [c, c + E) of a row.
 template <typename T, int E>
@@ -288,21 +303,28 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
   const float inv = bad || tiny ? 0.f : 127.f / r.top;
   const float hi = fmaf(inv, 4.76837158203125e-07f, inv), lo = fmaf(inv, -4.76837158203125e-07f, inv);
   uint32_t unsure = tiny && r.top > 0.f ? FULL_MASK : 0u;  // vectors to be done again
+  const bool alone = sizeof(T) == 2 && !(FULL && P.w) && free_of_127<T>(r.top);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * G + lane) * E;
     if (c >= d) break;
-    float w[FULL ? E : 1];
-    if constexpr (FULL) load_weights<T, E>(P, c, d, w);
-    uint32_t n[E], differ = 0;
+    [[maybe_unused]] float w[FULL ? E : 1];
+    uint32_t n[E];
+    if (alone) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      float t = RowType<T>::get(v[k].e[i]);
-      if constexpr (FULL) t *= w[i];
-      n[i] = __float_as_uint(fmaf(t, hi, ROUNDER));
-      differ |= n[i] ^ __float_as_uint(fmaf(t, lo, ROUNDER));
+      for (int i = 0; i < E; ++i) n[i] = __float_as_uint(fmaf(RowType<T>::get(v[k].e[i]), hi, ROUNDER));
+    } else {
+      if constexpr (FULL) load_weights<T, E>(P, c, d, w);
+      uint32_t differ = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        float t = RowType<T>::get(v[k].e[i]);
+        if constexpr (FULL) t *= w[i];
+        n[i] = __float_as_uint(fmaf(t, hi, ROUNDER));
+        differ |= n[i] ^ __float_as_uint(fmaf(t, lo, ROUNDER));
+      }
+      if (differ) unsure |= 1u << k;
     }
-    if (differ) unsure |= 1u << k;
     store_codes<E>(out, c, n, bad);
   }
   if (unsure && !bad) {
@@ -376,10 +398,12 @@ __global__ void __launch_bounds__(256) k_dequantize_rows(const __grid_constant__
 
 // ---------------------------------------------------------------- host side
 // Lanes a row and vectors a lane.  Many rows: the fewest lanes (8, 16, 32) that
-// hold the row in at most 8 vectors each.  Few rows (less than four warps an SM
-// with a warp a row) are latency: a warp each, from 4 vectors a lane on a block
-// of 128 or 512.  Rows that are not whole 16-byte vectors on 16 bytes go element
-// by element, neighbouring lanes on neighbouring elements.
+// hold the row in at most 8 vectors each, with a norm at most 4 (it has more in
+// flight and in registers; 64M bf16 values in rows of 1,024: 32 x 4 77 us, 16 x 8 86;
+// plain fp32 rows of 256: 8 x 8 50, 32 x 2 67).  Few rows (less than four warps an SM
+// with a warp a row) are latency: a warp each, from 4 vectors a lane on a block of
+// 128 or 512.  Rows that are not whole 16-byte vectors on 16 bytes go element by
+// element, neighbouring lanes on neighbouring elements.
 constexpr int64_t FEW_ROWS = 148 * 4;
 
 template <typename T, int E, int G, int NV, bool FULL>
@@ -409,12 +433,13 @@ static void quantize(const QuantizeParams& P, bool wide, cudaStream_t st) {
   } else if (vectors <= 8) launch_quantize<T, V, 8, 1, FULL>(P, st);
   else if (vectors <= 16) launch_quantize<T, V, 8, 2, FULL>(P, st);
   else if (vectors <= 32) launch_quantize<T, V, 8, 4, FULL>(P, st);
-  else if (vectors <= 48) launch_quantize<T, V, 8, 6, FULL>(P, st);
-  else if (vectors <= 64) launch_quantize<T, V, 8, 8, FULL>(P, st);
-  else if (vectors <= 96) launch_quantize<T, V, 16, 6, FULL>(P, st);
-  else if (vectors <= 128) launch_quantize<T, V, 16, 8, FULL>(P, st);
+  else if (vectors <= 48) launch_quantize<T, V, FULL ? 16 : 8, FULL ? 3 : 6, FULL>(P, st);
+  else if (vectors <= 64) launch_quantize<T, V, FULL ? 16 : 8, FULL ? 4 : 8, FULL>(P, st);
+  else if (vectors <= 96) launch_quantize<T, V, FULL ? 32 : 16, FULL ? 3 : 6, FULL>(P, st);
+  else if (vectors <= 128) launch_quantize<T, V, FULL ? 32 : 16, FULL ? 4 : 8, FULL>(P, st);
   else if (vectors <= 192) launch_quantize<T, V, 32, 6, FULL>(P, st);
   else if (vectors <= 256) launch_quantize<T, V, 32, 8, FULL>(P, st);
+  else if (vectors <= 384) launch_quantize<T, V, 128, 3, FULL>(P, st);
   else if (vectors <= 512) launch_quantize<T, V, 128, 4, FULL>(P, st);
   else if (vectors <= 1024) launch_quantize<T, V, 128, 8, FULL>(P, st);
   else if (vectors <= 2048) launch_quantize<T, V, 512, 4, FULL>(P, st);
