@@ -78,33 +78,34 @@ __device__ __forceinline__ void raise_top(float& top, const T (&v)[E]) {
   }
 }
 
-// E elements of a row held by one thread: a 16-byte vector (rows on 16 bytes, of
-// whole vectors) or a single element (any row).
+// A word of BYTES bytes.
+template <int BYTES>
+struct Word;
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<1> { using type = uint8_t; };
+
+// E elements of a row held by one thread, loaded and stored as one word: rows are
+// of whole words on their alignment.
 template <typename T, int E>
 struct Vec {
+  using W = typename Word<E * (int)sizeof(T)>::type;
   T e[E];
   // elements [c, c + E) of a row of d; zeros past its end
   __device__ __forceinline__ static Vec load(const T* row, int c, int d) {
+    W word{};
+    if (c < d) word = *reinterpret_cast<const W*>(row + c);
     Vec v;
-    if constexpr (E == 1) {
-      v.e[0] = RowType<T>::put(0.f);
-      if (c < d) v.e[0] = row[c];
-    } else {
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (c < d) raw = *reinterpret_cast<const uint4*>(row + c);
-      memcpy(&v, &raw, 16);
-    }
+    memcpy(&v, &word, sizeof(W));
     return v;
   }
   __device__ __forceinline__ void store(T* row, int c, int d) const {
     if (c >= d) return;
-    if constexpr (E == 1) {
-      row[c] = e[0];
-    } else {
-      uint4 raw;
-      memcpy(&raw, this, 16);
-      *reinterpret_cast<uint4*>(row + c) = raw;
-    }
+    W word;
+    memcpy(&word, this, sizeof(W));
+    *reinterpret_cast<W*>(row + c) = word;
   }
 };
 

@@ -129,7 +129,7 @@ __device__ __forceinline__ void load_weights(const QuantizeParams& P, int c, int
 #pragma unroll
     for (int i = 0; i < E; ++i) w[i] = 1.f;
   } else if (P.w_f32) {
-    constexpr int S = E == 1 ? 1 : 4;
+    constexpr int S = E < 4 ? E : 4;
 #pragma unroll
     for (int i = 0; i < E; i += S) {
       const auto b = Vec<float, S>::load(reinterpret_cast<const float*>(P.w), c + i, d);
@@ -146,19 +146,16 @@ __device__ __forceinline__ void load_weights(const QuantizeParams& P, int c, int
 // The codes n[i] & 255 of elements [c, c + E).
 template <int E>
 __device__ __forceinline__ void store_codes(int8_t* out, int c, const uint32_t (&n)[E], bool bad) {
-  if constexpr (E == 1) {
-    out[c] = bad ? 0 : (int8_t)n[0];
-  } else {
-    uint32_t q[E / 4];
+  uint32_t q[(E + 3) / 4];
 #pragma unroll
-    for (int i = 0; i < E / 4; ++i) {
-      q[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040),
-                         0x5410);
-      if (bad) q[i] = 0;
-    }
-    if constexpr (E == 4) *reinterpret_cast<uint32_t*>(out + c) = q[0];
-    else *reinterpret_cast<uint2*>(out + c) = make_uint2(q[0], q[1]);
+  for (int i = 0; i < (E + 3) / 4; ++i) {
+    q[i] = E == 1 ? n[0] : __byte_perm(n[4 * i], n[E == 1 ? 0 : 4 * i + 1], 0x0040);
+    if constexpr (E >= 4) q[i] = __byte_perm(q[i], __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040), 0x5410);
+    if (bad) q[i] = 0;
   }
+  typename Word<E>::type word;
+  memcpy(&word, q, E);
+  *reinterpret_cast<typename Word<E>::type*>(out + c) = word;
 }
 
 // Rare: the scale of a row whose squares leave the range of 32 bits, from
@@ -238,6 +235,9 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
 #pragma unroll
   for (int k = 0; k < NV; ++k) v[k] = Vec<T, E>::load(x, (k * G + lane) * E, d);
   RowSums r{0.f, 0.f, 0.f};
+  // products of narrow words are kept, those of wide ones (64 a thread) are made twice
+  constexpr bool KEEP = FULL && E <= 2;
+  [[maybe_unused]] float kept[KEEP ? NV : 1][E];
   if constexpr (FULL) {
     if (P.res) {
       const T* res = reinterpret_cast<const T*>(P.res) + (live ? row : 0) * P.res_stride;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
     for (int k = 0; k < NV; ++k) {
       float w[E];
       load_weights<T, E>(P, (k * G + lane) * E, d, w);
-      float u[E];
+      float(&u)[E] = KEEP ? kept[k % (KEEP ? NV : 1)] : kept[0];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const float e = RowType<T>::get(v[k].e[i]);
@@ -314,12 +314,13 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
 #pragma unroll
       for (int i = 0; i < E; ++i) n[i] = __float_as_uint(fmaf(RowType<T>::get(v[k].e[i]), hi, ROUNDER));
     } else {
-      if constexpr (FULL) load_weights<T, E>(P, c, d, w);
+      if constexpr (FULL && !KEEP) load_weights<T, E>(P, c, d, w);
       uint32_t differ = 0;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         float t = RowType<T>::get(v[k].e[i]);
-        if constexpr (FULL) t *= w[i];
+        if constexpr (KEEP) t = kept[k % NV][i];
+        else if constexpr (FULL) t *= w[i];
         n[i] = __float_as_uint(fmaf(t, hi, ROUNDER));
         differ |= n[i] ^ __float_as_uint(fmaf(t, lo, ROUNDER));
       }
@@ -368,15 +369,8 @@ __global__ void __launch_bounds__(256) k_dequantize_rows(const __grid_constant__
 #pragma unroll
       for (int j = 0; j < (E + 3) / 4; ++j) w[k][j] = 0;
       if (c < dk) {
-        if constexpr (E == 1) {
-          w[k][0] = (uint32_t)(uint8_t)__ldg(in + c);
-        } else if constexpr (E == 4) {
-          w[k][0] = __ldg(reinterpret_cast<const uint32_t*>(in + c));
-        } else {
-          const uint2 b = __ldg(reinterpret_cast<const uint2*>(in + c));
-          w[k][0] = b.x;
-          w[k][1] = b.y;
-        }
+        const typename Word<E>::type word = __ldg(reinterpret_cast<const typename Word<E>::type*>(in + c));
+        memcpy(w[k], &word, E);
       }
     }
 #pragma unroll
@@ -411,16 +405,37 @@ static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
   constexpr int threads = row_threads(G), rows = threads / G;
   k_quantize_rows<T, E, G, NV, FULL><<<(unsigned)((P.n + rows - 1) / rows), threads, 0, st>>>(P);
 }
+// Rows of narrower words than 16 bytes: neighbouring lanes on neighbouring words.
+template <typename T, int E, bool FULL>
+static void quantize_fine(const QuantizeParams& P, cudaStream_t st) {
+  const int words = P.d / E;
+  if (P.n <= FEW_ROWS) {
+    if (words <= 128) launch_quantize<T, E, 32, 4, FULL>(P, st);
+    else if (words <= 512) launch_quantize<T, E, 32, 16, FULL>(P, st);
+    else if (words <= 1024) launch_quantize<T, E, 128, 8, FULL>(P, st);
+    else if (words <= 4096) launch_quantize<T, E, 512, 8, FULL>(P, st);
+    else if (words <= 8192) launch_quantize<T, E, 512, 16, FULL>(P, st);
+    else if constexpr (E == 1) launch_quantize<T, E, 512, 32, FULL>(P, st);
+  } else if (words <= 32) launch_quantize<T, E, 4, 8, FULL>(P, st);
+  else if (words <= 64) launch_quantize<T, E, 8, 8, FULL>(P, st);
+  else if (words <= 128) launch_quantize<T, E, 8, 16, FULL>(P, st);
+  else if (words <= 256) launch_quantize<T, E, 16, 16, FULL>(P, st);
+  else if (words <= 512) launch_quantize<T, E, 32, 16, FULL>(P, st);
+  else if (words <= 1024) launch_quantize<T, E, FULL ? 128 : 32, FULL ? 8 : 32, FULL>(P, st);
+  else if (words <= 2048) launch_quantize<T, E, 128, 16, FULL>(P, st);
+  else if (words <= 4096) launch_quantize<T, E, 256, 16, FULL>(P, st);
+  else if (words <= 8192) launch_quantize<T, E, 512, 16, FULL>(P, st);
+  else if constexpr (E == 1) launch_quantize<T, E, 512, 32, FULL>(P, st);
+}
+// bytes: the widest word (16, or less) that the rows are whole words of.
 template <typename T, bool FULL>
-static void quantize(const QuantizeParams& P, bool wide, cudaStream_t st) {
+static void quantize(const QuantizeParams& P, int bytes, cudaStream_t st) {
   constexpr int V = RowType<T>::V;
-  if (!wide) {
-    if (P.d <= 128) launch_quantize<T, 1, 32, 4, FULL>(P, st);
-    else if (P.d <= 512) launch_quantize<T, 1, 32, 16, FULL>(P, st);
-    else if (P.d <= 1024) launch_quantize<T, 1, 32, 32, FULL>(P, st);
-    else if (P.d <= 4096) launch_quantize<T, 1, 128, 32, FULL>(P, st);
-    else launch_quantize<T, 1, 512, 32, FULL>(P, st);
-    return;
+  if (bytes < 16) {
+    if constexpr (V == 8) {
+      if (bytes >= 4) return quantize_fine<T, 2, FULL>(P, st);
+    }
+    return quantize_fine<T, 1, FULL>(P, st);
   }
   const int vectors = P.d / V;
   if (P.n <= FEW_ROWS && vectors > 8) {
@@ -430,8 +445,9 @@ static void quantize(const QuantizeParams& P, bool wide, cudaStream_t st) {
     else if (vectors <= 512) launch_quantize<T, V, 128, 4, FULL>(P, st);
     else if (vectors <= 2048) launch_quantize<T, V, 512, 4, FULL>(P, st);
     else if constexpr (V == 4) launch_quantize<T, V, 512, 8, FULL>(P, st);
-  } else if (vectors <= 8) launch_quantize<T, V, 8, 1, FULL>(P, st);
-  else if (vectors <= 16) launch_quantize<T, V, 8, 2, FULL>(P, st);
+  } else if (vectors <= 4) launch_quantize<T, V, 4, 1, FULL>(P, st);
+  else if (vectors <= 8) launch_quantize<T, V, 4, 2, FULL>(P, st);
+  else if (vectors <= 16) launch_quantize<T, V, 4, 4, FULL>(P, st);
   else if (vectors <= 32) launch_quantize<T, V, 8, 4, FULL>(P, st);
   else if (vectors <= 48) launch_quantize<T, V, FULL ? 16 : 8, FULL ? 3 : 6, FULL>(P, st);
   else if (vectors <= 64) launch_quantize<T, V, FULL ? 16 : 8, FULL ? 4 : 8, FULL>(P, st);
@@ -442,7 +458,7 @@ static void quantize(const QuantizeParams& P, bool wide, cudaStream_t st) {
   else if (vectors <= 384) launch_quantize<T, V, 128, 3, FULL>(P, st);
   else if (vectors <= 512) launch_quantize<T, V, 128, 4, FULL>(P, st);
   else if (vectors <= 1024) launch_quantize<T, V, 128, 8, FULL>(P, st);
-  else if (vectors <= 2048) launch_quantize<T, V, 512, 4, FULL>(P, st);
+  else if (vectors <= 2048) launch_quantize<T, V, 256, 8, FULL>(P, st);
   else if constexpr (V == 4) launch_quantize<T, V, 512, 8, FULL>(P, st);
 }
 
@@ -451,12 +467,26 @@ static void launch_read(const ReadParams& P, cudaStream_t st) {
   constexpr int rows = 256 / G;
   k_dequantize_rows<T, E, G, NV><<<(unsigned)((P.n + rows - 1) / rows), 256, 0, st>>>(P);
 }
+template <typename T, int E>
+static void read_fine(const ReadParams& P, cudaStream_t st) {
+  const int words = P.d / E;
+  if (words <= 32) launch_read<T, E, 4, 8>(P, st);
+  else if (words <= 64) launch_read<T, E, 8, 8>(P, st);
+  else if (words <= 128) launch_read<T, E, 16, 8>(P, st);
+  else launch_read<T, E, 32, 8>(P, st);
+}
 template <typename T>
-static void dequantize(const ReadParams& P, bool wide, cudaStream_t st) {
+static void dequantize(const ReadParams& P, int bytes, cudaStream_t st) {
   constexpr int V = RowType<T>::V;
   const int vectors = P.d / V;
-  if (!wide) launch_read<T, 1, 32, 8>(P, st);
-  else if (vectors <= 8) launch_read<T, V, 8, 1>(P, st);
+  if (bytes < 16) {
+    if constexpr (V == 8) {
+      if (bytes >= 4) return read_fine<T, 2>(P, st);
+    }
+    return read_fine<T, 1>(P, st);
+  }
+  if (vectors <= 4) launch_read<T, V, 4, 1>(P, st);
+  else if (vectors <= 8) launch_read<T, V, 4, 2>(P, st);
   else if (P.n <= FEW_ROWS) launch_read<T, V, 32, 4>(P, st);
   else if (vectors <= 16) launch_read<T, V, 8, 2>(P, st);
   else if (vectors <= 32) launch_read<T, V, 8, 4>(P, st);
@@ -521,11 +551,14 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
   P.inv_n = norm == CIRCUIT_NORM_RMS ? 1.f / (float)dim : 1.f;
   P.eps = eps;
   P.slot64 = slot_bytes == 8;
-  // whole 16-byte vectors, each one access
-  const int vec = 16 / e;
-  const bool wide = dim % vec == 0 && on16(rows, row_stride * e) &&
-                    (!residual || (on16(residual, residual_stride * e) && on16(summed, summed_stride * e))) &&
-                    on16(weight, 0) && ((uintptr_t)codes | (uintptr_t)code_stride) % vec == 0;
+  // the widest words that every row is made of; a code word is a byte for each value
+  uintptr_t bits = 16 | (uintptr_t)rows | (uintptr_t)(row_stride * e) | (uintptr_t)(dim * (int64_t)e) |
+                   ((uintptr_t)codes | (uintptr_t)code_stride) * e;
+  if (weight && weight_dtype == dtype) bits |= (uintptr_t)weight;
+  else if (weight && !on16(weight, 0)) bits |= (uintptr_t)weight % 8 ? 2 : 4;  // fp32 beside 16-bit words
+  if (residual)
+    bits |= (uintptr_t)residual | (uintptr_t)(residual_stride * e) | (uintptr_t)summed | (uintptr_t)(summed_stride * e);
+  const int bytes = (int)(bits & -bits);
   cudaStream_t st = (cudaStream_t)stream;
   // Equal slots: each row of a short write looks through the later ones; a long
   // write claims its slots first, the claims standing in the scales.
@@ -536,9 +569,9 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
     k_claim_slots<<<blocks, 256, 0, st>>>(slots, P.slot64, n, capacity, scales);
   }
   const bool full = norm != CIRCUIT_NORM_NONE;
-  if (dtype == CIRCUIT_F32) full ? quantize<float, true>(P, wide, st) : quantize<float, false>(P, wide, st);
-  else if (dtype == CIRCUIT_F16) full ? quantize<__half, true>(P, wide, st) : quantize<__half, false>(P, wide, st);
-  else full ? quantize<__nv_bfloat16, true>(P, wide, st) : quantize<__nv_bfloat16, false>(P, wide, st);
+  if (dtype == CIRCUIT_F32) full ? quantize<float, true>(P, bytes, st) : quantize<float, false>(P, bytes, st);
+  else if (dtype == CIRCUIT_F16) full ? quantize<__half, true>(P, bytes, st) : quantize<__half, false>(P, bytes, st);
+  else full ? quantize<__nv_bfloat16, true>(P, bytes, st) : quantize<__nv_bfloat16, false>(P, bytes, st);
   return check(cudaGetLastError(), "quantize_rows launch");
 }
 
@@ -557,12 +590,13 @@ int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const f
   if ((uintptr_t)out % e || (uintptr_t)scales % 4 || (ids && (uintptr_t)ids % id_bytes))
     return bad("dequantize_rows: a pointer is not aligned to its type");
   const ReadParams P{codes, scales, ids, out, n, rows, code_stride, out_stride, dim, id_bytes == 8};
-  const int vec = 16 / e;
-  const bool wide = dim % vec == 0 && on16(out, out_stride * e) && ((uintptr_t)codes | (uintptr_t)code_stride) % vec == 0;
+  const uintptr_t bits = 16 | (uintptr_t)out | (uintptr_t)(out_stride * e) | (uintptr_t)(dim * (int64_t)e) |
+                         ((uintptr_t)codes | (uintptr_t)code_stride) * e;
+  const int bytes = (int)(bits & -bits);  // the widest words that every row is made of
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == CIRCUIT_F32) dequantize<float>(P, wide, st);
-  else if (dtype == CIRCUIT_F16) dequantize<__half>(P, wide, st);
-  else dequantize<__nv_bfloat16>(P, wide, st);
+  if (dtype == CIRCUIT_F32) dequantize<float>(P, bytes, st);
+  else if (dtype == CIRCUIT_F16) dequantize<__half>(P, bytes, st);
+  else dequantize<__nv_bfloat16>(P, bytes, st);
   return check(cudaGetLastError(), "dequantize_rows launch");
 }
 
