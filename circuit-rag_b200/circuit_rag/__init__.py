@@ -8,8 +8,8 @@ there is no CPU search path.
 from circuit_rag.hierarchy.build import CircuitIndex, build_circuit_index
 from circuit_rag.search import circuit_search, circuit_search_batch, SearchTrace
 from circuit_rag.rag import CircuitRAG, SearchResult
-from circuit_rag.int8 import dequantize_rows, int8_scores, quantize_rows, rms_norm_quantize
+from circuit_rag.int8 import Int8Rows, dequantize_rows, int8_scores, quantize_rows, rms_norm_quantize
 
 __version__ = "0.1.0"
 __all__ = ["CircuitRAG", "SearchResult", "CircuitIndex", "build_circuit_index", "circuit_search", "circuit_search_batch",
-           "SearchTrace", "quantize_rows", "rms_norm_quantize", "dequantize_rows", "int8_scores"]
+           "SearchTrace", "Int8Rows", "quantize_rows", "rms_norm_quantize", "dequantize_rows", "int8_scores"]

@@ -78,3 +78,103 @@ def int8_scores(query_codes: torch.Tensor, query_scales: torch.Tensor, codes: to
     only contiguous where n allows); ``out`` may have any row stride.  Codes whose rows do not start on 16 bytes or end without padding are copied first;
     those of quantize_rows and Int8Rows never are."""
     return _bind().scores(query_codes, query_scales, codes, scales, bias, dtype, out)
+
+
+class Int8Rows:
+    """A store of 8-bit rows on one device: places that hold a row or none.
+
+    ``codes`` [len, dim] and ``scales`` [len] are what int8_scores and dequantize_rows take; a place without a row has
+    scale NaN, reads as NaN and is never a search result.  Calls on one store are ordered by their streams: writing
+    places while another stream reads them is the caller's to order."""
+
+    def __init__(self, places: int, dim: int, device="cuda"):
+        if not 1 <= dim <= _native.CIRCUIT_INT8_MAX_DIM or not 0 <= places < 2 ** 31:
+            raise ValueError(f"places must be in [0, 2^31) and dim in [1, {_native.CIRCUIT_INT8_MAX_DIM}]")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError("8-bit rows live on a CUDA device (no CPU path)")
+        self.dim = int(dim)
+        self._len = int(places)
+        self._codes, self._scales = self._buffers(self._len)
+
+    def _buffers(self, n: int):
+        codes = torch.zeros((n, (self.dim + 15) // 16 * 16), dtype=torch.int8, device=self.device)
+        return codes, torch.full((n,), float("nan"), dtype=torch.float32, device=self.device)
+
+    def __len__(self) -> int:
+        return self._len
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes[:self._len, :self.dim]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales[:self._len]
+
+    def write(self, rows: torch.Tensor, slots: torch.Tensor, normalize: bool = False) -> None:
+        """Quantises rows [n, dim] into places slots [n] (int32 or int64).  A slot outside the store writes nothing, of
+        equal slots the last row stays."""
+        quantize_rows(rows, slots=slots, out=(self.codes, self.scales), normalize=normalize)
+
+    def append(self, rows: torch.Tensor, normalize: bool = False) -> range:
+        """Adds rows [n, dim] in new places at the end and returns these places."""
+        if not isinstance(rows, torch.Tensor) or rows.ndim != 2 or rows.shape[1] != self.dim:
+            raise ValueError("rows must have shape [n, dim]")
+        first, need = self._len, self._len + rows.shape[0]
+        if need >= 2 ** 31:
+            raise ValueError("a store holds less than 2^31 rows")
+        if need > self._codes.shape[0]:
+            codes, scales = self._buffers(max(need, 2 * self._codes.shape[0]))
+            codes[:first].copy_(self._codes[:first])
+            scales[:first].copy_(self._scales[:first])
+            self._codes, self._scales = codes, scales
+        quantize_rows(rows, out=(self._codes[first:need, :self.dim], self._scales[first:need]), normalize=normalize)
+        self._len = need
+        return range(first, need)
+
+    def remove(self, slots: torch.Tensor) -> None:
+        """Empties the places ``slots`` (all inside the store)."""
+        self.scales[slots.to(device=self.device, dtype=torch.int64)] = float("nan")
+
+    def read(self, ids: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The rows at ``ids`` (any shape, as a search returns them; -1 gives zeros)."""
+        return dequantize_rows(self.codes, self.scales, ids, dtype=dtype)
+
+    def scores(self, queries: torch.Tensor, bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float32,
+               normalize: bool = False) -> torch.Tensor:
+        """Products [nq, len] of queries [nq, dim], quantised row by row, with all places."""
+        codes, scales = quantize_rows(queries, normalize=normalize)
+        return int8_scores(codes, scales, self.codes, self.scales, bias=bias, dtype=dtype)
+
+    def search(self, queries: torch.Tensor, k: int = 10, normalize: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The k best places of each query [nq, dim] by its product with the stored rows: (scores [nq, k] descending,
+        ids [nq, k] int32), ties to the lower place, score -inf and id -1 where there are fewer rows; 1 <= k <= 256."""
+        return self.search_codes(*quantize_rows(queries, normalize=normalize), k=k)
+
+    # scores of a block of rows that are ranked at a time
+    _BLOCK = 1 << 25
+
+    def search_codes(self, query_codes: torch.Tensor, query_scales: torch.Tensor, k: int = 10):
+        """search with queries that are quantised already."""
+        if not 1 <= int(k) <= _native.CIRCUIT_MAX_K:
+            raise ValueError(f"k must be in [1, {_native.CIRCUIT_MAX_K}]")
+        nq, n = query_codes.shape[0], self._len
+        none = -(1 << 63)
+        best = torch.full((nq, k), none, dtype=torch.int64, device=self.device)
+        block = max(1 << 14, self._BLOCK // max(1, nq))
+        for a in range(0, n if nq else 0, block):
+            b = min(n, a + block)
+            s = int8_scores(query_codes, query_scales, self._codes[a:b, :self.dim], self._scales[a:b])
+            # one whole number a score: the order of floats in the upper half, the lower place first in the lower half
+            bits = s.view(torch.int32).to(torch.int64)
+            bits ^= (bits >> 31) & 0x7FFFFFFF
+            key = (bits << 32) + (0xFFFFFFFF - torch.arange(a, b, device=self.device))
+            key.masked_fill_(s.isnan(), none)
+            best = torch.cat([best, key], 1).topk(k, dim=1).values
+        empty = best == none
+        bits = best >> 32
+        bits ^= (bits >> 31) & 0x7FFFFFFF
+        scores = bits.to(torch.int32).view(torch.float32).masked_fill_(empty, float("-inf"))
+        ids = (0xFFFFFFFF - (best & 0xFFFFFFFF)).to(torch.int32).masked_fill_(empty, -1)
+        return scores, ids

@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 from circuit_rag.hierarchy.build import build_circuit_index
+from circuit_rag.int8 import Int8Rows, rms_norm_quantize
 from circuit_rag.search import circuit_search
 
 
@@ -26,7 +27,11 @@ class SearchResult:
 
 class CircuitRAG:
     def __init__(self, embedding_model: str = "BAAI/bge-small-en-v1.5", device: Optional[str] = None,
-                 embed_fn: Optional[Callable[[List[str]], np.ndarray]] = None):
+                 embed_fn: Optional[Callable[[List[str]], np.ndarray]] = None, rows: str = "float32"):
+        if rows not in ("float32", "int8"):
+            raise ValueError('rows must be "float32" or "int8"')
+        self.rows = rows
+        self.store: Optional[Int8Rows] = None
         self.device = device or ("cuda" if torch.cuda.is_available() else "cpu")
         if embed_fn is None:
             from sentence_transformers import SentenceTransformer  # optional dependency
@@ -59,6 +64,14 @@ class CircuitRAG:
             raise ValueError("metadatas must be the same length as texts")
         new_vecs = np.asarray(self._embed(texts), dtype=np.float32)
         start_id = len(self.texts)
+        if self.rows == "int8":
+            if self.store is None:
+                self.store = Int8Rows(0, new_vecs.shape[1], self.device)
+            # unit length: scores are cosines
+            self.store.append(torch.from_numpy(new_vecs).to(self.store.device), normalize=True)
+            self.texts.extend(texts)
+            self.metadatas.extend(metadatas)
+            return list(range(start_id, len(self.texts)))
         self.texts.extend(texts)
         self.metadatas.extend(metadatas)
         if self._vectors is None:
@@ -82,10 +95,33 @@ class CircuitRAG:
         self._built_n = n
         self.appended_rows = 0
 
-    def search(self, query: str, k: int = 5) -> List[SearchResult]:
-        if self.index is None:
+    def search(self, query: str, k: int = 5, feedback: Optional[List[int]] = None) -> List[SearchResult]:
+        """The k best documents (reference rag.py:57-65).  feedback (8-bit rows only): ids of documents found
+        relevant; the query (at unit length) is moved by their mean before it is compared."""
+        if feedback and self.rows != "int8":
+            raise ValueError('feedback needs rows="int8"')
+        if self.index is None and self.store is None:
             return []
         q = torch.from_numpy(np.asarray(self._embed([query]), dtype=np.float32)[0])
-        scores, ids, _ = circuit_search(q, self.index, k=min(k, len(self.texts)))
+        k = min(k, len(self.texts))
+        if self.rows == "int8":
+            scores, ids = self._search_rows(q.to(self.store.device)[None], k, feedback or [])
+        else:
+            scores, ids, _ = circuit_search(q, self.index, k=k)
         return [SearchResult(id=int(i), score=float(s), text=self.texts[int(i)], metadata=self.metadatas[int(i)])
-                for s, i in zip(scores.tolist(), ids.tolist())]
+                for s, i in zip(scores.tolist(), ids.tolist()) if i >= 0]
+
+    def _search_rows(self, q: torch.Tensor, k: int, feedback: List[int]):
+        if any(not 0 <= i < len(self.texts) for i in feedback):
+            raise ValueError("feedback must be ids of documents")
+        if feedback:
+            ids = torch.tensor(feedback, dtype=torch.int64, device=q.device)
+            mean = self.store.read(ids).mean(0, keepdim=True)
+            q = q / q.norm().clamp(min=torch.finfo(q.dtype).tiny)  # as long as each document
+            # the root-mean-square norm times dim^-1/2: unit length again
+            unit = torch.full((self.store.dim,), self.store.dim ** -0.5, device=q.device)
+            codes, scales, _ = rms_norm_quantize(q, residual=mean, weight=unit, eps=0.0)
+            scores, found = self.store.search_codes(codes, scales, k=k)
+        else:
+            scores, found = self.store.search(q, k=k, normalize=True)
+        return scores[0], found[0]

@@ -88,3 +88,16 @@ def test_python_refuses_cpu_tensors():
 def test_symbols_have_signatures():
     for name in ("circuit_op_quantize_rows", "circuit_op_dequantize_rows", "circuit_op_int8_scores"):
         assert getattr(_native.lib(), name).restype is ctypes.c_int
+
+
+def test_rag_refuses_8_bit_rows_on_the_cpu():
+    from circuit_rag import CircuitRAG
+
+    with pytest.raises(ValueError):
+        CircuitRAG(device="cpu", embed_fn=len, rows="int4")
+    rag = CircuitRAG(device="cpu", embed_fn=lambda texts: np.ones((len(texts), 4), np.float32), rows="int8")
+    with pytest.raises(RuntimeError):
+        rag.add_documents(["a"])
+    assert rag.texts == [] and rag.search("a") == []
+    with pytest.raises(ValueError):
+        CircuitRAG(device="cpu", embed_fn=len).search("a", feedback=[1])
