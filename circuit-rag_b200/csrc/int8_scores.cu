@@ -72,16 +72,21 @@ __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
 // (its N); units are dealt round robin with the query tiles fastest, so a row
 // tile comes from HBM once and its other query tiles read it from L2.  A TMA warp
 // streams 128-byte K chunks of both operands through a 192 KB ring, one elected
-// thread issues the MMAs into one of two TMEM accumulators, and four or eight
-// epilogue warps scale the other one.  With rows as M, a lane of the accumulator is a row
+// thread issues the MMAs into one of two to eight TMEM accumulators, and sixteen
+// epilogue warps scale the others.  With rows as M, a lane of the accumulator is a row
 // and a column a query: each warp store writes 32 consecutive results of one
 // query's row of `out`, without a transposition.
 constexpr int MMA_ROWS = 128;
-// Epilogue warps: a result is an integer conversion (a quarter-rate instruction: 2,048
-// clocks for a 128 x 256 tile), two products, an address and a store, so a tile's
-// results take many warps to keep pace; then a TMA and an MMA warp.
-constexpr int epilogue_warps(int BN) { return BN >= 256 ? 16 : BN >= 64 ? 8 : 4; }
-constexpr int mma_threads(int BN) { return (epilogue_warps(BN) + 2) * 32; }
+// Epilogue warps: four cover a tile's 128 TMEM lanes and `parts` of them its columns; for
+// few queries `groups` of them take turns with the tiles, since what a small tile
+// costs is the way from the MMA through the accumulator to the stores (about 1,800
+// clocks with one group and two accumulators), not its results.  Then a TMA and an
+// MMA warp.
+constexpr int EPILOGUE_WARPS = 16;
+constexpr int MMA_THREADS = (EPILOGUE_WARPS + 2) * 32;
+constexpr int column_parts(int BN) { return BN <= 64 ? 1 : BN / 64; }
+constexpr int tile_groups(int BN) { return EPILOGUE_WARPS / 4 / column_parts(BN); }
+constexpr int accumulators(int BN) { return BN <= 64 ? 8 : 512 / BN; }
 
 // Units first, first + step, ... as (row tile, query tile), query tiles fastest,
 // without a division a unit.
@@ -157,16 +162,17 @@ __device__ __forceinline__ void store_columns(char* out, uint32_t ld, int64_t ld
   }
 }
 
-// An epilogue warp's loop over its units: 32 rows of the tile (its TMEM lanes) from
-// row_off on, COLS columns.  The next unit's scales and the next 16 columns are on
-// their way while the present ones are stored.  Once a wait has given up, the
-// results that it would have brought are NaN.
-template <typename T, int COLS, typename Release>
-__device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, int BN, float* sq, Units un,
-                                         int64_t units, int tile_rows, int row_off, uint64_t* acc_full,
-                                         Release release) {
+// An epilogue warp's loop over its group's units: 32 rows of the tile (its TMEM
+// lanes) from row_off on, COLS columns.  The next unit's scales and the next 16
+// columns are on their way while the present ones are stored.  Once a wait has given
+// up, the results that it would have brought are NaN.
+template <typename T, int BN, typename Release>
+__device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, float* sq, Units un, int64_t units,
+                                         int tile_rows, int row_off, uint64_t* acc_full, Release release) {
+  constexpr int PARTS = column_parts(BN), GROUPS = tile_groups(BN), NB = accumulators(BN), COLS = BN / PARTS;
   constexpr int W = 16, N = COLS / W, SQ = (COLS + 31) / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, part = warp >> 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
+  const int part = (warp >> 2) % PARTS, group = (warp >> 2) / PARTS;
   const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(part * COLS);
   const int64_t ld64 = P.out_stride * (int64_t)sizeof(T);
   const uint32_t ld = ld64 < (1ll << 32) ? (uint32_t)ld64 : 0u;
@@ -182,10 +188,11 @@ __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, i
     for (int i = 0; i < SQ; ++i)
       sqv[i] = 32 * i + lane < COLS && q0 + 32 * i + lane < P.nq ? __ldg(P.q_scales + q0 + 32 * i + lane) : 0.f;
   };
+  for (int i = 0; i < group; ++i) un.next();
   if (un.u < units) fetch();
   bool ok = true;
-  for (int it = 0; un.u < units; ++it) {
-    const int b = it & 1;
+  for (int it = group; un.u < units; it += GROUPS) {
+    const int b = it % NB;
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < SQ; ++i)
@@ -196,9 +203,10 @@ __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, i
     char* out = reinterpret_cast<char*>(P.out) + q0 * ld64 + row * (int64_t)sizeof(T);
     float s = sr;
     const float bb = bias;
-    un.next();
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) un.next();
     if (un.u < units) fetch();
-    ok = ok && __all_sync(FULL_MASK, mbar_wait(&acc_full[b], (uint32_t)(it / 2) & 1u, &g_error, ERR_TIMEOUT_FULL));
+    ok = ok && __all_sync(FULL_MASK, mbar_wait(&acc_full[b], (uint32_t)(it / NB) & 1u, &g_error, ERR_TIMEOUT_FULL));
     if (!ok) s = __uint_as_float(0x7fffffffu);
     tc::fence_after();
     uint32_t v[2][W];
@@ -213,24 +221,25 @@ __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, i
         __syncwarp();
         if (lane == 0) release(b);
       }
-      store_columns<T, W>(out + i * W * ld64, ld, ld64, v[i & 1], sq + i * W, s, bb, row < P.n, left - i * W, pairs);
+      if (i * W < left)
+        store_columns<T, W>(out + i * W * ld64, ld, ld64, v[i & 1], sq + i * W, s, bb, row < P.n, left - i * W, pairs);
     }
   }
   return ok;
 }
 
 template <typename T, int BN>
-__global__ void __launch_bounds__(mma_threads(BN), 1)
+__global__ void __launch_bounds__(MMA_THREADS, 1)
     k_scores_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
                  int q_tiles, int64_t units) {
-  constexpr int S = ring_stages(BN), STAGE = chunk_bytes(BN), EW = epilogue_warps(BN), COLS = BN / (EW / 4);
+  constexpr int S = ring_stages(BN), STAGE = chunk_bytes(BN), EW = EPILOGUE_WARPS, NB = accumulators(BN);
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[S], empty[S], acc_full[NB], acc_empty[NB];
   __shared__ uint32_t tmem_base;
   __shared__ int s_failed;
-  __shared__ __align__(16) float s_sq[EW][COLS];
+  __shared__ __align__(16) float s_sq[EW][BN / column_parts(BN)];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunks = (P.d + 127) >> 7;
   if (threadIdx.x == 0) {
@@ -238,14 +247,14 @@ __global__ void __launch_bounds__(mma_threads(BN), 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < NB; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], EW);  // one lane of each epilogue warp
+      mbar_init(&acc_empty[b], 4 * column_parts(BN));  // one lane of each epilogue warp of a group
     }
     s_failed = 0;
     fence_mbar_init();
   }
-  if (warp == EW + 1) tc::tmem_alloc(&tmem_base, 2 * BN);
+  if (warp == EW + 1) tc::tmem_alloc(&tmem_base, NB * BN);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -282,8 +291,8 @@ __global__ void __launch_bounds__(mma_threads(BN), 1)
     uint32_t ph = 0;
     bool ok = true;
     for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++it) {
-      const int b = it & 1;
-      if (it >= 2 && !__all_sync(FULL_MASK, mbar_wait(&acc_empty[b], (uint32_t)(it / 2 - 1) & 1u, &g_error,
+      const int b = it % NB;
+      if (it >= NB && !__all_sync(FULL_MASK, mbar_wait(&acc_empty[b], (uint32_t)(it / NB - 1) & 1u, &g_error,
                                                       ERR_TIMEOUT_EMPTY))) {
         ok = false;
         break;
@@ -309,14 +318,14 @@ __global__ void __launch_bounds__(mma_threads(BN), 1)
     }
     if (!ok && lane == 0) s_failed = 1;
   } else {
-    const bool ok = epilogue<T, COLS>(P, tmem, BN, s_sq[warp], Units(blockIdx.x, gridDim.x, q_tiles), units, MMA_ROWS, 0,
+    const bool ok = epilogue<T, BN>(P, tmem, s_sq[warp], Units(blockIdx.x, gridDim.x, q_tiles), units, MMA_ROWS, 0,
                                       acc_full, [&](int b) { mbar_arrive(&acc_empty[b]); });
     if (!ok && lane == 0) s_failed = 1;
   }
   tc::fence_before();
   __syncthreads();
   if (s_failed) grace_period();  // copies and MMAs of the failed waits end before the memory is freed
-  if (warp == EW + 1) tc::tmem_dealloc(tmem, 2 * BN);
+  if (warp == EW + 1) tc::tmem_dealloc(tmem, NB * BN);
 }
 
 // The same for many queries with a CTA pair a unit of 256 rows x 256 queries: each
@@ -327,13 +336,13 @@ __global__ void __launch_bounds__(mma_threads(BN), 1)
 constexpr int PAIR_BN = 256;
 constexpr int PAIR_STAGE = (MMA_ROWS + PAIR_BN / 2) * 128;
 constexpr int PAIR_STAGES = RING_BYTES / PAIR_STAGE;
-constexpr int PAIR_EW = epilogue_warps(PAIR_BN);
 
 template <typename T>
-__global__ void __launch_bounds__(mma_threads(PAIR_BN), 1)
+__global__ void __launch_bounds__(MMA_THREADS, 1)
     k_scores_pair(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
                   int q_tiles, int64_t units) {
-  constexpr int S = PAIR_STAGES, EW = PAIR_EW, COLS = PAIR_BN / (EW / 4);
+  constexpr int S = PAIR_STAGES, EW = EPILOGUE_WARPS;
+  static_assert(accumulators(PAIR_BN) == 2 && tile_groups(PAIR_BN) == 1, "two accumulators, every warp on every tile");
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -341,7 +350,7 @@ __global__ void __launch_bounds__(mma_threads(PAIR_BN), 1)
   __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   __shared__ int s_failed;
-  __shared__ __align__(16) float s_sq[EW][COLS];
+  __shared__ __align__(16) float s_sq[EW][PAIR_BN / column_parts(PAIR_BN)];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunks = (P.d + 127) >> 7;
   const uint32_t rank = tc::cluster_ctarank();
@@ -435,7 +444,7 @@ __global__ void __launch_bounds__(mma_threads(PAIR_BN), 1)
       if (!ok && lane == 0) s_failed = 1;
     }
   } else {
-    const bool ok = epilogue<T, COLS>(P, tmem, PAIR_BN, s_sq[warp], Units(first, step, q_tiles), units, 2 * MMA_ROWS,
+    const bool ok = epilogue<T, PAIR_BN>(P, tmem, s_sq[warp], Units(first, step, q_tiles), units, 2 * MMA_ROWS,
                                       (int)rank * MMA_ROWS, acc_full,
                                       [&](int b) { tc::mbar_arrive_remote(lead_acc_empty + 8u * (uint32_t)b); });
     if (!ok && lane == 0) s_failed = 1;
@@ -487,7 +496,7 @@ static int launch_mma(const ScoresParams& P, cudaStream_t st) {
   if (rc) return rc;
   const int q_tiles = (int)((P.nq + BN - 1) / BN);
   const int64_t units = (P.n + MMA_ROWS - 1) / MMA_ROWS * q_tiles, sms = sm_count();
-  k_scores_mma<T, BN><<<(unsigned)(units < sms ? units : sms), mma_threads(BN), smem, st>>>(qmap, cmap, P, q_tiles, units);
+  k_scores_mma<T, BN><<<(unsigned)(units < sms ? units : sms), MMA_THREADS, smem, st>>>(qmap, cmap, P, q_tiles, units);
   return CIRCUIT_OK;
 }
 
@@ -522,7 +531,7 @@ static int launch_pair(const ScoresParams& P, cudaStream_t st) {
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(2 * (units < pairs ? units : pairs)));
-  cfg.blockDim = dim3(mma_threads(PAIR_BN));
+  cfg.blockDim = dim3(MMA_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = &cluster;
