@@ -106,9 +106,30 @@ struct Units {
     }
   }
 };
+
 constexpr int RING_BYTES = 192 * 1024;
+// Rows in flight: 96 KB an SM is best (2M rows of 384, one query: 3 / 4 / 5 / 6 / 8 / 12 stages of 16 KB take 146 /
+// 129 / 123 / 117 / 117 / 123 us; 32 queries: 184 / 163 / 158 / 153 / 160 / 172); beside many results 80 KB
+// (100 queries: 73 / 67 / 68 / 74 / 80 / 80).
+constexpr int MAX_STAGES = 6;
 constexpr int chunk_bytes(int BN) { return (MMA_ROWS + BN) * 128; }
-constexpr int ring_stages(int BN) { return RING_BYTES / chunk_bytes(BN); }
+
+// The shared memory of a CTA: stages of a K chunk of rows (and of the queries); with a
+// single query tile for several row tiles a CTA its queries stand behind the stages for
+// good, as far as they leave half of the memory: loading the same few lines again for every row tile, from
+// every SM at once, cost more than the rows themselves.
+struct Ring {
+  int stages, bn;
+  bool resident;
+  __host__ __device__ int stage_bytes() const { return resident ? MMA_ROWS * 128 : chunk_bytes(bn); }
+  static Ring of(int bn, int chunks, bool many_rows) {
+    Ring r{0, bn, many_rows && chunks * bn * 128 <= RING_BYTES / 2};
+    const int n = (RING_BYTES - (r.resident ? chunks * bn * 128 : 0)) / r.stage_bytes();
+    const int most = bn < 128 ? MAX_STAGES : MAX_STAGES - 1;
+    r.stages = n < most ? n : most;
+    return r;
+  }
+};
 
 // Bits of the waits that gave up, kept until circuit_op_int8_status reads them.
 __device__ int g_error;
@@ -231,12 +252,13 @@ __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, f
 template <typename T, int BN>
 __global__ void __launch_bounds__(MMA_THREADS, 1)
     k_scores_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
-                 int q_tiles, int64_t units) {
-  constexpr int S = ring_stages(BN), STAGE = chunk_bytes(BN), EW = EPILOGUE_WARPS, NB = accumulators(BN);
+                 int q_tiles, int64_t units, Ring ring) {
+  constexpr int EW = EPILOGUE_WARPS, NB = accumulators(BN);
+  const int S = ring.stages, STAGE = ring.stage_bytes();
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[S], empty[S], acc_full[NB], acc_empty[NB];
+  __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[NB], acc_empty[NB], q_full;
   __shared__ uint32_t tmem_base;
   __shared__ int s_failed;
   __shared__ __align__(16) float s_sq[EW][BN / column_parts(BN)];
@@ -251,6 +273,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 4 * column_parts(BN));  // one lane of each epilogue warp of a group
     }
+    mbar_init(&q_full, 1);
     s_failed = 0;
     fence_mbar_init();
   }
@@ -266,6 +289,10 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
       int64_t filled = 0;
       uint32_t ph = 0;
       bool ok = true;
+      if (ring.resident) {
+        mbar_arrive_expect_tx(&q_full, (uint32_t)(chunks * BN * 128));
+        for (int j = 0; j < chunks; ++j) tc::tma_load_2d(smem + S * STAGE + j * BN * 128, &qmap, 128 * j, 0, &q_full);
+      }
       for (Units un(blockIdx.x, gridDim.x, q_tiles); un.u < units && ok; un.next()) {
         const int row0 = (int)(un.rt * MMA_ROWS), q0 = un.qt * BN;
         for (int j = 0; j < chunks; ++j, ++filled) {
@@ -273,7 +300,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
           mbar_arrive_expect_tx(&full[s], STAGE);  // out-of-range rows and columns arrive as zeros
           unsigned char* dst = smem + s * STAGE;
           tc::tma_load_2d(dst, &cmap, 128 * j, row0, &full[s]);
-          tc::tma_load_2d(dst + MMA_ROWS * 128, &qmap, 128 * j, q0, &full[s]);
+          if (!ring.resident) tc::tma_load_2d(dst + MMA_ROWS * 128, &qmap, 128 * j, q0, &full[s]);
           if (++s == S) { s = 0; ph ^= 1u; }
         }
       }
@@ -285,11 +312,13 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
   } else if (warp == EW + 1) {
     constexpr uint32_t idesc = tc::idesc_s8(MMA_ROWS, BN);
     const uint32_t sbase = smem_u32(smem);
-    const uint64_t dA = tc::sdesc_k_sw128(sbase), dB = tc::sdesc_k_sw128(sbase + MMA_ROWS * 128);
+    // the chunk's queries: beside its rows in the stage, or chunk by chunk behind the ring
+    const uint64_t dA = tc::sdesc_k_sw128(sbase),
+                   dB = tc::sdesc_k_sw128(sbase + (ring.resident ? S * STAGE : MMA_ROWS * 128));
     const int tail = (P.d - (chunks - 1) * 128 + 31) >> 5;  // K steps of 32 in the last chunk
     int s = 0, it = 0;
     uint32_t ph = 0;
-    bool ok = true;
+    bool ok = !ring.resident || __all_sync(FULL_MASK, mbar_wait(&q_full, 0u, &g_error, ERR_TIMEOUT_FULL));
     for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++it) {
       const int b = it % NB;
       if (it >= NB && !__all_sync(FULL_MASK, mbar_wait(&acc_empty[b], (uint32_t)(it / NB - 1) & 1u, &g_error,
@@ -303,11 +332,12 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
         if (!__all_sync(FULL_MASK, mbar_wait(&full[s], ph, &g_error, ERR_TIMEOUT_FULL))) { ok = false; break; }
         tc::fence_after();
         if (tc::elect_one()) {
-          const uint64_t off = (uint64_t)((uint32_t)(s * STAGE) >> 4);
+          const uint64_t a = dA + ((uint32_t)(s * STAGE) >> 4);
+          const uint64_t q = dB + ((uint32_t)(ring.resident ? j * BN * 128 : s * STAGE) >> 4);
           const int steps = j + 1 < chunks ? 4 : tail;
 #pragma unroll
           for (int k = 0; k < 4; ++k)  // 32 bytes of K further: 2 units of 16 bytes
-            if (k < steps) tc::mma_s8_ss(acc, dA + off + 2 * k, dB + off + 2 * k, idesc, (j | k) != 0 ? 1u : 0u);
+            if (k < steps) tc::mma_s8_ss(acc, a + 2 * k, q + 2 * k, idesc, (j | k) != 0 ? 1u : 0u);
           tc::commit(&empty[s]);
         }
         __syncwarp();
@@ -340,14 +370,14 @@ constexpr int PAIR_STAGES = RING_BYTES / PAIR_STAGE;
 template <typename T>
 __global__ void __launch_bounds__(MMA_THREADS, 1)
     k_scores_pair(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
-                  int q_tiles, int64_t units) {
-  constexpr int S = PAIR_STAGES, EW = EPILOGUE_WARPS;
+                  int q_tiles, int64_t units, int S) {
+  constexpr int EW = EPILOGUE_WARPS;
   static_assert(accumulators(PAIR_BN) == 2 && tile_groups(PAIR_BN) == 1, "two accumulators, every warp on every tile");
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   // full and acc_empty are used in the even CTA only, empty and acc_full in both
-  __shared__ uint64_t full[S], empty[S], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base;
   __shared__ int s_failed;
   __shared__ __align__(16) float s_sq[EW][PAIR_BN / column_parts(PAIR_BN)];
@@ -490,13 +520,14 @@ static int launch_mma(const ScoresParams& P, cudaStream_t st) {
   CUtensorMap qmap, cmap;
   if (!code_map(&qmap, P.q, P.nq, P.d, P.q_stride, BN) || !code_map(&cmap, P.codes, P.n, P.d, P.code_stride, MMA_ROWS))
     return bad("int8_scores: cuTensorMapEncodeTiled refused the code rows");
-  constexpr int smem = ring_stages(BN) * chunk_bytes(BN) + 1024;
+  constexpr int smem = RING_BYTES + 1024;
   const int rc = check(cudaFuncSetAttribute(k_scores_mma<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
                        "int8_scores shared memory");
   if (rc) return rc;
   const int q_tiles = (int)((P.nq + BN - 1) / BN);
   const int64_t units = (P.n + MMA_ROWS - 1) / MMA_ROWS * q_tiles, sms = sm_count();
-  k_scores_mma<T, BN><<<(unsigned)(units < sms ? units : sms), MMA_THREADS, smem, st>>>(qmap, cmap, P, q_tiles, units);
+  k_scores_mma<T, BN><<<(unsigned)(units < sms ? units : sms), MMA_THREADS, smem, st>>>(qmap, cmap, P, q_tiles, units,
+                                                                              Ring::of(BN, (P.d + 127) / 128, q_tiles == 1 && units > 2 * sms));
   return CIRCUIT_OK;
 }
 
@@ -536,7 +567,10 @@ static int launch_pair(const ScoresParams& P, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
-  return check(cudaLaunchKernelEx(&cfg, k_scores_pair<T>, qmap, cmap, P, q_tiles, units), "int8_scores launch");
+  // short sums are bound by the results' way out, which less in flight disturbs less (200,000 x 100 fp16, 558 queries: 4
+  // stages 63 us, 6 stages 69; 1,024 x 40,000 x 768: 34 and 31)
+  const int stages = P.d <= 512 ? 4 : PAIR_STAGES;
+  return check(cudaLaunchKernelEx(&cfg, k_scores_pair<T>, qmap, cmap, P, q_tiles, units, stages), "int8_scores launch");
 }
 
 template <typename T>
