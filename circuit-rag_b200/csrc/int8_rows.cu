@@ -63,20 +63,18 @@ __device__ __forceinline__ RowSums reduce(RowSums r) {
 // nearest integer.  u, top and the division are off by 2^-24 of their size each and
 // hi and lo by another, so the real quotient lies between u * lo and u * hi: where
 // both give the same integer it is the code, where not (within 127 2^-21 = 6e-5 of
-// a half: 0.006 % of the values) the quotient is taken in 64 bits, in which v * w
-// is exact.
+// a half: 0.006 % of the values) 254 v w is compared with (2 n + 1) top in 64 bits,
+// in which v * w is exact.
 //
 // 16-bit values without a weight have m < 2^11 steps of their exponent, as has top
 // (ma): 127 v / top = 127 mv / (ma 2^k) is either a half, or 1 / (2 ma 2^k) >=
 // 2^-19 of its size away from one, more than hi's 10 * 2^-24.  A half needs 254 mv =
 // (2 n + 1) ma 2^k, so the prime 127 divides 2 n + 1 (which is then 127: v = top / 2,
 // a value that 16-bit rows often hold, and n = 63 goes to the even 64, as u * hi says)
-// or ma.  So hi alone gives the code unless 127 divides ma.
+// or ma.  So hi alone gives the code unless 127 divides ma.  The one such significand
+// of bf16, 254, makes 127 / top a power of two, which alone gives the code, halves
+// (every second value there) to even; the eight of fp16 take the general way.
 constexpr float ROUNDER = 12582912.f;
-__device__ __forceinline__ int code_near_half(float v, float w, double a) {
-  return (int)rint((double)v * (double)w * 127.0 / a);
-}
-
 // Whether 127 does not divide the significand of a 16-bit value's magnitude.
 template <typename T>
 __device__ __forceinline__ bool free_of_127(float top) {
@@ -178,13 +176,25 @@ __device__ __noinline__ float wide_range_scale(const T* src, int d, float top, f
   return (float)((double)top / 127.0 / sqrt(ldexp((double)m.ss * (double)inv_n, 2 * e) + (double)eps));
 }
 
-// Rare: codes of elements [c, c + e) from the 64-bit quotient.
+// Rare: codes of elements [c, c + e), halves decided in 64 bits (a: the row's exact
+// maximum; hi = 0: the row is too small for 32 bits throughout).
 template <typename T>
-__device__ __noinline__ void exact_codes(const QuantizeParams& P, const T* src, int8_t* out, int c, int e, double a) {
+__device__ __noinline__ void exact_codes(const QuantizeParams& P, const T* src, int8_t* out, int c, int e, double a,
+                                         float hi, float lo) {
   for (int i = c; i < c + e; ++i) {
     float w = 1.f;
     if (P.w) w = P.w_f32 ? reinterpret_cast<const float*>(P.w)[i] : RowType<T>::get(reinterpret_cast<const T*>(P.w)[i]);
-    out[i] = (int8_t)code_near_half(RowType<T>::get(src[i]), w, a);
+    const float v = RowType<T>::get(src[i]), t = v * w;
+    const double u = fabs((double)v * (double)w);
+    int n;
+    if (hi == 0.f) {
+      n = (int)rint(u * 127.0 / a);
+    } else {
+      const int n0 = (int)(fmaf(fabsf(t), lo, ROUNDER) - ROUNDER), n1 = (int)(fmaf(fabsf(t), hi, ROUNDER) - ROUNDER);
+      const double above = 254.0 * u - (double)(2 * n0 + 1) * a;
+      n = n0 == n1 ? n0 : above > 0.0 ? n1 : above < 0.0 ? n0 : n0 + (n0 & 1);
+    }
+    out[i] = (int8_t)(t < 0.f ? -n : n);
   }
 }
 
@@ -303,7 +313,9 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
   const float inv = bad || tiny ? 0.f : 127.f / r.top;
   const float hi = fmaf(inv, 4.76837158203125e-07f, inv), lo = fmaf(inv, -4.76837158203125e-07f, inv);
   uint32_t unsure = tiny && r.top > 0.f ? FULL_MASK : 0u;  // vectors to be done again
-  const bool alone = sizeof(T) == 2 && !(FULL && P.w) && free_of_127<T>(r.top);
+  const bool free = sizeof(T) == 2 && free_of_127<T>(r.top);
+  const bool alone = sizeof(T) == 2 && !(FULL && P.w) && (std::is_same<T, __nv_bfloat16>::value || free);
+  const float one = free ? hi : inv;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * G + lane) * E;
@@ -312,7 +324,7 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
     uint32_t n[E];
     if (alone) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) n[i] = __float_as_uint(fmaf(RowType<T>::get(v[k].e[i]), hi, ROUNDER));
+      for (int i = 0; i < E; ++i) n[i] = __float_as_uint(fmaf(RowType<T>::get(v[k].e[i]), one, ROUNDER));
     } else {
       if constexpr (FULL && !KEEP) load_weights<T, E>(P, c, d, w);
       uint32_t differ = 0;
@@ -333,7 +345,7 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
     for (int k = 0; k < NV; ++k)
       if (unsure >> k & 1u) {
         const int c = (k * G + lane) * E;
-        if (c < d) exact_codes<T>(P, x, out, c, E, a);
+        if (c < d) exact_codes<T>(P, x, out, c, E, a, hi, lo);
       }
   }
 }
@@ -473,7 +485,8 @@ static void read_fine(const ReadParams& P, cudaStream_t st) {
   if (words <= 32) launch_read<T, E, 4, 8>(P, st);
   else if (words <= 64) launch_read<T, E, 8, 8>(P, st);
   else if (words <= 128) launch_read<T, E, 16, 8>(P, st);
-  else launch_read<T, E, 32, 8>(P, st);
+  else if (words <= 256 || (words <= 1024 && P.n > FEW_ROWS)) launch_read<T, E, 32, 8>(P, st);
+  else launch_read<T, E, 256, 8>(P, st);
 }
 template <typename T>
 static void dequantize(const ReadParams& P, int bytes, cudaStream_t st) {
@@ -487,7 +500,7 @@ static void dequantize(const ReadParams& P, int bytes, cudaStream_t st) {
   }
   if (vectors <= 4) launch_read<T, V, 4, 1>(P, st);
   else if (vectors <= 8) launch_read<T, V, 4, 2>(P, st);
-  else if (P.n <= FEW_ROWS) launch_read<T, V, 32, 4>(P, st);
+  else if (P.n <= FEW_ROWS && vectors <= 128) launch_read<T, V, 32, 4>(P, st);
   else if (vectors <= 16) launch_read<T, V, 8, 2>(P, st);
   else if (vectors <= 32) launch_read<T, V, 8, 4>(P, st);
   else if (vectors <= 48) launch_read<T, V, 8, 6>(P, st);
@@ -495,7 +508,8 @@ static void dequantize(const ReadParams& P, int bytes, cudaStream_t st) {
   else if (vectors <= 96) launch_read<T, V, 16, 6>(P, st);
   else if (vectors <= 128) launch_read<T, V, 16, 8>(P, st);
   else if (vectors <= 192) launch_read<T, V, 32, 6>(P, st);
-  else launch_read<T, V, 32, 8>(P, st);
+  else if (vectors <= 256) launch_read<T, V, 32, 8>(P, st);
+  else launch_read<T, V, 256, 4>(P, st);
 }
 
 }  // namespace i8

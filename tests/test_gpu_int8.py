@@ -66,12 +66,25 @@ def test_quantize_strides_and_alignment(dtype):
         _check_plain(x, codes, scales)
 
 
-def test_quantize_ties_go_to_even():
-    x = torch.arange(-127, 128, device=DEV).repeat_interleave(2)[:508].float() / 2
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_ties_go_to_even(dtype):
+    # maxima of 127 times a power of two: every second value is a half; others: only top / 2 is
+    x = torch.arange(-127, 128, device=DEV).repeat_interleave(2)[:504].float() / 2
     x[-1] = 127.0
-    rows = torch.stack([x, x * 2.0 ** -20, -x])
-    codes, scales = quantize_rows(rows)
-    _check_plain(rows, codes, scales)
+    rows = torch.stack([x, x * 2.0 ** -7, -x, x / 2 ** 6]).to(dtype)
+    top = torch.tensor([1.0, 1.25, 127.0, 254.0, 190.5, 1.9921875, 3.0, 0.0078125], device=DEV)[:, None]
+    half = torch.cat([top, top / 2, -top / 2, top / 4, -top, torch.zeros_like(top), top / 2, top * 0.75], 1).to(dtype)
+    for y in (rows, rows.repeat(200, 1), half, half.repeat(300, 7), half.float(), torch.cat([half, half[:, :1]], 1)):
+        codes, scales = quantize_rows(y)
+        _check_plain(y, codes, scales)
+        codes, scales = quantize_rows(y, normalize=True)
+        _check_norm(y, None, None, 0.0, (codes, scales, None), unit=True)
+    # 16-bit rows of every significand of the maximum
+    g = torch.Generator(device=DEV).manual_seed(1)
+    bits = torch.arange(0, 2 ** 11, device=DEV)
+    top = (1 + bits / 2 ** 11).to(dtype)[:, None]
+    y = torch.cat([top, (torch.rand(2048, 255, generator=g, device=DEV) * top).to(dtype)], 1)
+    _check_plain(y, *quantize_rows(y))
 
 
 def test_quantize_next_to_halves():
@@ -87,10 +100,11 @@ def test_quantize_next_to_halves():
         _check_plain(x, codes, scales)
 
 
-@pytest.mark.parametrize("scale", [1e-44, 1e-40, 1e-38, 1e-30, 1e-18, 1e30, 1e37])
-def test_quantize_extreme_magnitudes(scale):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1e-44, 1e-40, 1e-38, 1e-30, 1e-18, 1e30, 1e36, 1e37])
+def test_quantize_extreme_magnitudes(scale, dtype):
     x = _rows(6, 260, torch.float32, seed=1)
-    x = (x.double() * scale).float()
+    x = (x.double() * scale).to(dtype)
     for y in (x, x[:, 1:], x.repeat(120, 1)):
         codes, scales = quantize_rows(y)
         _check_plain(y, codes, scales)
