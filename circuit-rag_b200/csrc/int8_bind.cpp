@@ -11,8 +11,8 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/add.h>
-#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -120,7 +120,7 @@ void check_target(const Tensor& t, const char* name) {
 }
 
 Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(dev));
+  return at::detail::empty_cuda(shape, type, dev, std::nullopt);
 }
 // New codes [n, dim] as a view of rows padded to a multiple of 16 bytes.
 Tensor fresh_codes(int64_t n, int64_t dim, const at::Device& dev) {

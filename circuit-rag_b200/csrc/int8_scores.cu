@@ -3,6 +3,9 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
+#include "engine.h"
 #include "int8.cuh"
 #include "tcgen05.cuh"
 
@@ -509,9 +512,12 @@ static bool code_map(CUtensorMap* map, const int8_t* base, int64_t rows, int d, 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 static int sm_count() {
+  static std::atomic<int> known[SmemOptIn::kMaxDevices];
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= SmemOptIn::kMaxDevices) return 148;
+  if ((n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -521,8 +527,8 @@ static int launch_mma(const ScoresParams& P, cudaStream_t st) {
   if (!code_map(&qmap, P.q, P.nq, P.d, P.q_stride, BN) || !code_map(&cmap, P.codes, P.n, P.d, P.code_stride, MMA_ROWS))
     return bad("int8_scores: cuTensorMapEncodeTiled refused the code rows");
   constexpr int smem = RING_BYTES + 1024;
-  const int rc = check(cudaFuncSetAttribute(k_scores_mma<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                       "int8_scores shared memory");
+  static SmemOptIn opt_in;
+  const int rc = check(opt_in.ensure(reinterpret_cast<const void*>(k_scores_mma<T, BN>), smem), "int8_scores shared memory");
   if (rc) return rc;
   const int q_tiles = (int)((P.nq + BN - 1) / BN);
   const int64_t units = (P.n + MMA_ROWS - 1) / MMA_ROWS * q_tiles, sms = sm_count();
@@ -533,12 +539,8 @@ static int launch_mma(const ScoresParams& P, cudaStream_t st) {
 
 template <typename T, int NQ>
 static int launch_rows(const ScoresParams& P, cudaStream_t st) {
+  static_assert(NQ * CIRCUIT_INT8_MAX_DIM <= 48 * 1024, "the queries fit the default shared memory");
   const int smem = NQ * ((P.d + 15) / 16) * 16;
-  if (smem > 48 * 1024) {
-    const int rc = check(cudaFuncSetAttribute(k_scores_rows<T, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                         "int8_scores shared memory");
-    if (rc) return rc;
-  }
   const int64_t blocks = (P.n + 31) / 32;
   const dim3 grid((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), (unsigned)((P.nq + NQ - 1) / NQ));
   k_scores_rows<T, NQ><<<grid, 256, smem, st>>>(P);
@@ -551,8 +553,8 @@ static int launch_pair(const ScoresParams& P, cudaStream_t st) {
       !code_map(&cmap, P.codes, P.n, P.d, P.code_stride, MMA_ROWS))
     return bad("int8_scores: cuTensorMapEncodeTiled refused the code rows");
   constexpr int smem = PAIR_STAGES * PAIR_STAGE + 1024;
-  const int rc = check(cudaFuncSetAttribute(k_scores_pair<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                       "int8_scores shared memory");
+  static SmemOptIn opt_in;
+  const int rc = check(opt_in.ensure(reinterpret_cast<const void*>(k_scores_pair<T>), smem), "int8_scores shared memory");
   if (rc) return rc;
   const int q_tiles = (int)((P.nq + PAIR_BN - 1) / PAIR_BN);
   const int64_t units = (P.n + 2 * MMA_ROWS - 1) / (2 * MMA_ROWS) * q_tiles, pairs = sm_count() / 2;
@@ -615,9 +617,14 @@ int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const fl
                        out_stride, dim,
                        e == 2 && ((uintptr_t)out & 3) == 0 && out_stride % 2 == 0};
   cudaStream_t st = (cudaStream_t)stream;
-  const int rc = dtype == CIRCUIT_F32   ? scores<float>(P, st)
-                 : dtype == CIRCUIT_F16 ? scores<__half>(P, st)
-                                        : scores<__nv_bfloat16>(P, st);
+  int rc = CIRCUIT_ERR_CUDA;
+  try {
+    rc = dtype == CIRCUIT_F32   ? scores<float>(P, st)
+         : dtype == CIRCUIT_F16 ? scores<__half>(P, st)
+                                : scores<__nv_bfloat16>(P, st);
+  } catch (...) {  // a lock of the host's that failed
+    return bad("int8_scores: the host ran out of a resource");
+  }
   return rc ? rc : check(cudaGetLastError(), "int8_scores launch");
 }
 
