@@ -113,6 +113,7 @@ void check_pair(const Tensor& codes, const Tensor& scales, const char* name) {
   if (scales.dim() != 1 || scales.scalar_type() != at::kFloat || scales.size(0) != codes.size(0))
     value_error(std::string(name) + " scales must be float32 of shape [n]");
   if (scales.device() != codes.device()) value_error(std::string(name) + " codes and scales must be on one device");
+  no_gradient(scales, name);
   check_dim(codes.size(1));
 }
 void check_target(const Tensor& t, const char* name) {
@@ -131,11 +132,11 @@ Tensor fresh_codes(int64_t n, int64_t dim, const at::Device& dev) {
   }
   return t;
 }
-// New results [nq, n] whose rows start on 128 bytes: a warp's 32 results then fill whole lines (a row length off
-// that takes the product kernel 1.7 times as long).
+// New results [nq, n]; those of 256 rows and more start their rows on 128 bytes: a warp's 32 results then fill whole
+// lines (a row length off that takes the product kernel 1.7 times as long).
 Tensor fresh_results(int64_t nq, int64_t n, at::ScalarType type, const at::Device& dev) {
   const int64_t line = 128 / (int64_t)c10::elementSize(type), ld = (n + line - 1) / line * line;
-  if (nq < 2 || ld == n) return fresh({nq, n}, type, dev);
+  if (nq < 2 || n < 256 || ld == n) return fresh({nq, n}, type, dev);
   Tensor t = fresh({nq, ld}, type, dev);
   const int64_t sizes[2] = {nq, n}, strides[2] = {ld, 1};
   t.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef(sizes), at::IntArrayRef(strides));

@@ -28,8 +28,10 @@ __device__ __forceinline__ float result(int acc, float sq, float sr, float bias)
   return fmaf((float)acc * sq, sr, bias);
 }
 
-// Eight lanes a row, each with 16 codes a step, NQ queries in shared memory
-// (zero past d, so what a row's padding holds does not count).
+// ---------------------------------------------------------------- few bytes
+// One or two queries against few rows: latency.  Eight lanes a row, each with 16
+// codes a step, the queries in shared memory (zero past d, so what a row's padding
+// holds does not count).
 template <typename T, int NQ>
 __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
   extern __shared__ __align__(16) int8_t s_q[];
@@ -74,7 +76,7 @@ __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
 // One persistent CTA an SM.  A unit is 128 rows (the MMA's M) against BN queries
 // (its N); units are dealt round robin with the query tiles fastest, so a row
 // tile comes from HBM once and its other query tiles read it from L2.  A TMA warp
-// streams 128-byte K chunks of both operands through a 192 KB ring, one elected
+// streams 128-byte K chunks of both operands through a ring of stages, one elected
 // thread issues the MMAs into one of two to eight TMEM accumulators, and sixteen
 // epilogue warps scale the others.  With rows as M, a lane of the accumulator is a row
 // and a column a query: each warp store writes 32 consecutive results of one
@@ -111,16 +113,17 @@ struct Units {
 };
 
 constexpr int RING_BYTES = 192 * 1024;
-// Rows in flight: 96 KB an SM is best (2M rows of 384, one query: 3 / 4 / 5 / 6 / 8 / 12 stages of 16 KB take 146 /
-// 129 / 123 / 117 / 117 / 123 us; 32 queries: 184 / 163 / 158 / 153 / 160 / 172); beside many results 80 KB
-// (100 queries: 73 / 67 / 68 / 74 / 80 / 80).
+// Rows in flight: 96 KB an SM is best (2M rows of 384, one query: 3 / 4 / 5 / 6 / 8 / 12
+// stages of 16 KB take 146 / 129 / 123 / 117 / 117 / 123 us; 32 queries: 184 / 163 / 158 /
+// 153 / 160 / 172); beside many results 80 KB (100 queries: 73 / 67 / 68 / 74 / 80 / 80).
 constexpr int MAX_STAGES = 6;
 constexpr int chunk_bytes(int BN) { return (MMA_ROWS + BN) * 128; }
 
 // The shared memory of a CTA: stages of a K chunk of rows (and of the queries); with a
 // single query tile for several row tiles a CTA its queries stand behind the stages for
-// good, as far as they leave half of the memory: loading the same few lines again for every row tile, from
-// every SM at once, cost more than the rows themselves.
+// good, as far as they leave half of the memory: loading the same few lines again for
+// every row tile, from every SM at once, cost more than the rows themselves
+// (922,893 rows of 42, 34 queries: 119 -> 40 us).
 struct Ring {
   int stages, bn;
   bool resident;
@@ -280,6 +283,10 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
     s_failed = 0;
     fence_mbar_init();
   }
+  if (threadIdx.x == 32 * EW) {
+    tc::prefetch_map(&cmap);
+    tc::prefetch_map(&qmap);
+  }
   if (warp == EW + 1) tc::tmem_alloc(&tmem_base, NB * BN);
   tc::fence_before();
   __syncthreads();
@@ -400,6 +407,10 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
     s_failed = 0;
     tc::fence_mbar_init_cluster();
     fence_mbar_init();
+  }
+  if (threadIdx.x == 32 * EW) {
+    tc::prefetch_map(&cmap);
+    tc::prefetch_map(&qmap);
   }
   if (warp == EW + 1) tc::tmem_alloc_pair(&tmem_base, 2 * PAIR_BN);
   tc::fence_before();

@@ -104,6 +104,10 @@ __device__ __forceinline__ void ld_32x32b_x16(uint32_t taddr, uint32_t (&v)[16])
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// Brings a tensor map (a kernel parameter) into the descriptor cache ahead of its first use.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // 2-D tiled TMA load: box at (x = inner element index, y = row) into smem.
 __device__ __forceinline__ void tma_load_2d(void* dst_smem, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(

@@ -471,3 +471,74 @@ def test_together_on_a_side_stream_and_in_a_graph(nq):
 
 def test_no_wait_has_given_up():
     assert _native.lib().circuit_op_int8_status(None) == 0
+
+
+def test_layout_of_new_results():
+    qc, qs = _codes(5, 64, seed=1)
+    for n in (1, 255, 256, 300, 1000):
+        rc, rs = _codes(n, 64, seed=n)
+        for dtype in TYPES:
+            got = int8_scores(qc, qs, rc, rs, dtype=dtype)
+            _check_scores(got, qc, qs, rc, rs, None, dtype)
+            line = 128 // got.element_size()
+            assert got.stride() == (n if n < 256 else -(-n // line) * line, 1)
+    one = int8_scores(qc[:1], qs[:1], rc, rs)
+    assert one.is_contiguous() and one.shape == (1, 1000)
+
+
+def test_gradients_are_refused_everywhere():
+    x = _rows(4, 32, torch.float32)
+    codes, scales = quantize_rows(x)
+    wants = [t.clone().requires_grad_() for t in (x, x[0], scales)]
+    for call in (lambda: rms_norm_quantize(wants[0]), lambda: rms_norm_quantize(x, residual=wants[0]),
+                 lambda: rms_norm_quantize(x, weight=wants[1]), lambda: dequantize_rows(codes, wants[2]),
+                 lambda: int8_scores(codes, wants[2], codes, scales), lambda: int8_scores(codes, scales, codes, wants[2]),
+                 lambda: int8_scores(codes, scales, codes, scales, bias=wants[2]),
+                 lambda: quantize_rows(x, out=(codes, wants[2]))):
+        with pytest.raises(RuntimeError):
+            call()
+    with torch.no_grad():
+        int8_scores(codes, wants[2], codes, scales)
+
+
+def test_calls_of_two_streams_at_once():
+    """Products and writes of two stores on two streams, each as if it were alone."""
+    work = []
+    for seed in (1, 2):
+        x = _rows(3000, 512, torch.bfloat16, seed)
+        rc, rs = _codes(40000, 512, seed + 10)
+        qc, qs = _codes(200, 512, seed + 20)
+        _, codes, scales = _store(5000, 512, 0)
+        work.append((x, rc, rs, qc, qs, codes, scales, torch.randperm(5000, device=DEV)[:3000]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    got = [[], []]
+    for _ in range(5):
+        for k, (x, rc, rs, qc, qs, codes, scales, slots) in enumerate(work):
+            with torch.cuda.stream(streams[k]):
+                quantize_rows(x, slots=slots, out=(codes, scales))
+                got[k].append(int8_scores(qc, qs, rc, rs))
+    torch.cuda.synchronize()
+    for k, (x, rc, rs, qc, qs, codes, scales, slots) in enumerate(work):
+        _check_plain(x, codes[slots], scales[slots])
+        for s in got[k]:
+            assert torch.equal(s, got[k][0])
+        _check_scores(got[k][0], qc, qs, rc, rs, None, torch.float32)
+
+
+def test_norm_in_place_of_its_inputs():
+    """The C entry's sum may be the rows or the residual themselves."""
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 2)):
+        for d in (384, 385, 5000):
+            x, r, w = _rows(70, d, dtype, 1), _rows(70, d, dtype, 2), _rows(1, d, dtype, 3)[0]
+            x[5] *= 1e-30 if dtype == torch.float32 else 1
+            r[5] *= 1e-30 if dtype == torch.float32 else 1
+            for into in (0, 1):
+                pair = [x.clone(), r.clone()]
+                codes, scales = torch.empty(70, d + 3, dtype=torch.int8, device=DEV)[:, :d], torch.empty(70, device=DEV)
+                rc = _native.lib().circuit_op_quantize_rows(
+                    pair[0].data_ptr(), code, 70, d, d, pair[1].data_ptr(), d, w.data_ptr(), code, 1, 1e-6,
+                    pair[into].data_ptr(), d, None, 0, 70, codes.data_ptr(), d + 3, scales.data_ptr(),
+                    torch.cuda.current_stream().cuda_stream)
+                assert rc == 0
+                _check_norm(x, r, w, float(torch.tensor(1e-6)), (codes, scales, pair[into]))
