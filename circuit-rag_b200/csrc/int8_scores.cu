@@ -597,6 +597,13 @@ static int scores(const ScoresParams& P, cudaStream_t st) {
   if (P.nq <= 32) return launch_mma<T, 32>(P, st);
   if (P.nq <= 64) return launch_mma<T, 64>(P, st);
   if (P.nq <= 128) return launch_mma<T, 128>(P, st);
+  // Pairs of CTAs take 256 x 256 tiles, single ones 128 x 128: a round of pairs costs about one and a half rounds of
+  // single CTAs and does twice as much, when it is full (300 queries against 50,000 rows of 384: 6 rounds 22.6 us, 8
+  // single ones 16.5; 1,024 against 40,000 of 768: 9 rounds 31.8 us, 17 single ones 42.6).
+  const int64_t sms = sm_count(), pairs = sms / 2 > 0 ? sms / 2 : 1;
+  const int64_t single = ((P.n + 127) / 128 * ((P.nq + 127) / 128) + sms - 1) / sms;
+  const int64_t paired = ((P.n + 255) / 256 * ((P.nq + 255) / 256) + pairs - 1) / pairs;
+  if (2 * single < 3 * paired) return launch_mma<T, 128>(P, st);
   return launch_pair<T>(P, st);
 }
 

@@ -542,3 +542,16 @@ def test_norm_in_place_of_its_inputs():
                     torch.cuda.current_stream().cuda_stream)
                 assert rc == 0
                 _check_norm(x, r, w, float(torch.tensor(1e-6)), (codes, scales, pair[into]))
+
+
+@pytest.mark.parametrize("d", [20, 130, 384, 1000, 2500])
+@pytest.mark.parametrize("nq", [1, 3, 16, 17, 40, 64, 100, 128, 129, 256, 300, 500, 1000])
+def test_scores_of_many_rows(nq, d):
+    """Several row tiles a block, full and partial ones, in every kernel: the queries' tile kept, streamed, or paired."""
+    n = 60001
+    dtype = TYPES[(nq + d) % 3]
+    qc, qs = _codes(nq, d, seed=d + nq)
+    rc, rs = _codes(n, d, seed=d)
+    bias = torch.randn(n, device=DEV) if nq % 2 else None
+    out = None if d % 20 else torch.empty(nq, n, dtype=dtype, device=DEV)  # rows off 128 bytes
+    _check_scores(int8_scores(qc, qs, rc, rs, bias=bias, dtype=dtype, out=out), qc, qs, rc, rs, bias, dtype)
