@@ -406,11 +406,11 @@ __global__ void __launch_bounds__(256) k_dequantize_rows(const __grid_constant__
 // Lanes a row and vectors a lane.  Many rows: the fewest lanes (8, 16, 32) that
 // hold the row in at most 8 vectors each, with a norm at most 4 (it has more in
 // flight and in registers; 64M bf16 values in rows of 1,024: 32 x 4 77 us, 16 x 8 86;
-// plain fp32 rows of 256: 8 x 8 50, 32 x 2 67).  Few rows (less than four warps an SM
-// with a warp a row) are latency: a warp each, from 4 vectors a lane on a block of
-// 128 or 512.  Rows that are not whole 16-byte vectors on 16 bytes go element by
+// plain fp32 rows of 256: 8 x 8 50, 32 x 2 67).  Few rows (up to eight warps an SM with a
+// warp a row, two for the longest) are latency: a warp each, from 4 vectors a lane on a
+// block of 128 or 512 (700 fp32 rows of 1,024 with a norm: 4.8 us, 7.3 the other way).  Rows that are not whole 16-byte vectors on 16 bytes go element by
 // element, neighbouring lanes on neighbouring elements.
-constexpr int64_t FEW_ROWS = 148 * 4;
+constexpr int64_t FEW_ROWS = 148 * 8, FEW_LONG_ROWS = 148 * 2;
 
 template <typename T, int E, int G, int NV, bool FULL>
 static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
@@ -450,7 +450,7 @@ static void quantize(const QuantizeParams& P, int bytes, cudaStream_t st) {
     return quantize_fine<T, 1, FULL>(P, st);
   }
   const int vectors = P.d / V;
-  if (P.n <= FEW_ROWS && vectors > 8) {
+  if (vectors > 8 && P.n <= (vectors <= 512 ? FEW_ROWS : FEW_LONG_ROWS)) {
     if (vectors <= 32) launch_quantize<T, V, 32, 1, FULL>(P, st);
     else if (vectors <= 64) launch_quantize<T, V, 32, 2, FULL>(P, st);
     else if (vectors <= 128) launch_quantize<T, V, 32, 4, FULL>(P, st);
