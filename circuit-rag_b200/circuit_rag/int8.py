@@ -74,9 +74,10 @@ def int8_scores(query_codes: torch.Tensor, query_scales: torch.Tensor, codes: to
     """Products [nq, n] of 8-bit queries with 8-bit rows: query_scales[i] * scales[j] * (codes' inner product), plus
     bias[j] (float32 [n]: a prior of each row, or -|x|^2 / 2 for distances), rounded once to ``dtype``.
 
-    The sum over dim is exact.  A new result of 256 rows and more starts its rows on 128 bytes (its row stride is n
-    rounded up, so it is only contiguous where n allows); ``out`` may have any row stride.  Codes whose rows do not start on 16 bytes or end without padding are copied first;
-    those of quantize_rows and Int8Rows never are."""
+    The sum over dim is exact; times the query's scale it has to stay in the range of float32 (values up to 1e32).  A
+    new result of 256 rows and more starts its rows on 128 bytes (its row stride is n rounded up, so it is only
+    contiguous where n allows); ``out`` may have any row stride.  Codes whose rows do not start on 16 bytes or end
+    without padding are copied first; those of quantize_rows and Int8Rows never are."""
     return _bind().scores(query_codes, query_scales, codes, scales, bias, dtype, out)
 
 

@@ -5,6 +5,9 @@ scale has four more roundings and the fp32 sum of squares (at most 64 terms a th
 the error halves under the root): (4 + (64 + 9 + 1) / 2) 2^-24 < 2.5e-6 relative.  A read value is one fp32 product and
 one rounding to its type; a score three fp32 roundings and one to its type (a rounding: eps / 2)."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -50,7 +53,7 @@ DIMS = [1, 2, 7, 16, 31, 33, 64, 128, 136, 200, 256, 384, 385, 511, 512, 513, 64
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", DIMS)
 def test_quantize_dims(d, dtype):
-    for n in (1, 5, 67, 701):
+    for n in (1, 5, 67, 701, 1300):
         x = _rows(n, d, dtype, seed=d + n)
         codes, scales = quantize_rows(x)
         assert codes.shape == (n, d) and codes.dtype == torch.int8 and scales.dtype == torch.float32
@@ -150,7 +153,7 @@ def _check_norm(x, r, w, eps, got, unit=False):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", DIMS)
 def test_norm_dims(d, dtype):
-    for n in (1, 37, 613):
+    for n in (1, 37, 613, 1250):
         x, r = _rows(n, d, dtype, seed=d), _rows(n, d, dtype, seed=d + 1, scale=0.3)
         w = (1 + 0.2 * _rows(1, d, torch.float32, seed=d + 2)[0])
         for rr, ww in ((r, w.to(dtype)), (r, w), (None, w), (r, None), (None, None)):
@@ -555,3 +558,60 @@ def test_scores_of_many_rows(nq, d):
     bias = torch.randn(n, device=DEV) if nq % 2 else None
     out = None if d % 20 else torch.empty(nq, n, dtype=dtype, device=DEV)  # rows off 128 bytes
     _check_scores(int8_scores(qc, qs, rc, rs, bias=bias, dtype=dtype, out=out), qc, qs, rc, rs, bias, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [3, 16, 24, 33, 64, 100, 130, 384, 385, 514, 1000, 1030, 1100, 2500, 8200])
+def test_read_many_rows(d, dtype):
+    codes, scales = _codes(1500, d, seed=d)
+    ids = torch.randint(-1, 1500, (3000,), device=DEV)
+    want = torch.where((ids >= 0)[:, None], codes[ids].double() * scales[ids].double()[:, None], 0)
+    tol = U32 + _half(dtype)
+    for rows in (codes, codes.contiguous()):
+        got = dequantize_rows(rows, scales, ids, dtype=dtype)
+        assert ((got.double() - want).abs() <= tol * (1 + tol) * want.abs() + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("n", [700, 4000])
+@pytest.mark.parametrize("d", [24, 384, 385, 5000])
+def test_write_at_unit_length(n, d):
+    x = _rows(n, d, torch.float16, seed=d)
+    slots = torch.randint(0, n, (n,), generator=torch.Generator().manual_seed(1))
+    buf, codes, scales = _store(n, d)
+    quantize_rows(x, slots=slots.to(DEV), out=(codes, scales), normalize=True)
+    last = {s: i for i, s in enumerate(slots.tolist())}
+    at, row = torch.tensor(list(last), device=DEV), torch.tensor(list(last.values()), device=DEV)
+    _check_norm(x[row], None, None, 0.0, (codes[at], scales[at], None), unit=True)
+    left = torch.ones(n, dtype=torch.bool, device=DEV)
+    left[at] = False
+    assert (codes[left] == 77).all() and (scales[left] == -3.5).all()
+
+
+def test_first_calls_inside_a_capture():
+    """Nothing of the calls needs an eager one first: a fresh process captures them at once."""
+    code = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from circuit_rag.int8 import dequantize_rows, int8_scores, quantize_rows, rms_norm_quantize
+x, y = torch.randn(4000, 256, device="cuda"), torch.randn(300, 256, device="cuda")
+slots = torch.randperm(4000, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a = quantize_rows(x)
+    b = rms_norm_quantize(y, residual=y)
+    quantize_rows(x, slots=slots, out=a)
+    results = [int8_scores(b[0][:n], b[1][:n], *a) for n in (1, 16, 64, 128, 300)]
+    back = dequantize_rows(*a, slots)
+graph.replay()
+torch.cuda.synchronize()
+for r, n in zip(results, (1, 16, 64, 128, 300)):
+    want = (b[0][:n].double() @ a[0].double().T) * b[1][:n, None].double() * a[1].double()
+    torch.testing.assert_close(r.double(), want, rtol=1e-6, atol=0)
+assert torch.equal(back, a[0][slots].float() * a[1][slots][:, None])
+print("captured")
+"""
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "circuit-rag_b200")
+    done = subprocess.run([sys.executable, "-c", code, root], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
