@@ -91,7 +91,11 @@ constexpr int EPILOGUE_WARPS = 16;
 constexpr int MMA_THREADS = (EPILOGUE_WARPS + 2) * 32;
 constexpr int column_parts(int BN) { return BN <= 64 ? 1 : BN / 64; }
 constexpr int tile_groups(int BN) { return EPILOGUE_WARPS / 4 / column_parts(BN); }
-constexpr int accumulators(int BN) { return BN <= 64 ? 8 : 512 / BN; }
+// Accumulators of SUBS x BN columns in 512 columns of TMEM.  SUBS: 128-row tiles of a
+// unit.  A unit's way through the MMA warp (two waits, two commits) takes 800 clocks
+// however little it is, so with rows of one chunk two tiles go as one unit
+// (4M rows of 64, 8 queries: 107 -> 74 us).
+constexpr int accumulators(int BN, int SUBS = 1) { return 512 / (BN * SUBS) < 8 ? 512 / (BN * SUBS) : 8; }
 
 // Units first, first + step, ... as (row tile, query tile), query tiles fastest,
 // without a division a unit.
@@ -117,7 +121,6 @@ constexpr int RING_BYTES = 192 * 1024;
 // stages of 16 KB take 146 / 129 / 123 / 117 / 117 / 123 us; 32 queries: 184 / 163 / 158 /
 // 153 / 160 / 172); beside many results 80 KB (100 queries: 73 / 67 / 68 / 74 / 80 / 80).
 constexpr int MAX_STAGES = 6;
-constexpr int chunk_bytes(int BN) { return (MMA_ROWS + BN) * 128; }
 
 // The shared memory of a CTA: stages of a K chunk of rows (and of the queries); with a
 // single query tile for several row tiles a CTA its queries stand behind the stages for
@@ -125,13 +128,13 @@ constexpr int chunk_bytes(int BN) { return (MMA_ROWS + BN) * 128; }
 // every row tile, from every SM at once, cost more than the rows themselves
 // (922,893 rows of 42, 34 queries: 119 -> 40 us).
 struct Ring {
-  int stages, bn;
+  int stages, rows, bn;
   bool resident;
-  __host__ __device__ int stage_bytes() const { return resident ? MMA_ROWS * 128 : chunk_bytes(bn); }
-  static Ring of(int bn, int chunks, bool many_rows) {
-    Ring r{0, bn, many_rows && chunks * bn * 128 <= RING_BYTES / 2};
+  __host__ __device__ int stage_bytes() const { return (rows + (resident ? 0 : bn)) * 128; }
+  static Ring of(int rows, int bn, int chunks, bool many_rows) {
+    Ring r{0, rows, bn, many_rows && chunks * bn * 128 <= RING_BYTES / 2};
     const int n = (RING_BYTES - (r.resident ? chunks * bn * 128 : 0)) / r.stage_bytes();
-    const int most = bn < 128 ? MAX_STAGES : MAX_STAGES - 1;
+    const int most = (bn < 128 ? MAX_STAGES : MAX_STAGES - 1) * MMA_ROWS / rows;
     r.stages = n < most ? n : most;
     return r;
   }
@@ -193,20 +196,20 @@ __device__ __forceinline__ void store_columns(char* out, uint32_t ld, int64_t ld
 // lanes) from row_off on, COLS columns.  The next unit's scales and the next 16
 // columns are on their way while the present ones are stored.  Once a wait has given
 // up, the results that it would have brought are NaN.
-template <typename T, int BN, typename Release>
+template <typename T, int BN, int SUBS, typename Release>
 __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, float* sq, Units un, int64_t units,
                                          int tile_rows, int row_off, uint64_t* acc_full, Release release) {
-  constexpr int PARTS = column_parts(BN), GROUPS = tile_groups(BN), NB = accumulators(BN), COLS = BN / PARTS;
+  constexpr int PARTS = column_parts(BN), GROUPS = tile_groups(BN) / SUBS, NB = accumulators(BN, SUBS), COLS = BN / PARTS;
   constexpr int W = 16, N = COLS / W, SQ = (COLS + 31) / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
-  const int part = (warp >> 2) % PARTS, group = (warp >> 2) / PARTS;
-  const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(part * COLS);
+  const int part = (warp >> 2) % PARTS, sub = (warp >> 2) / PARTS % SUBS, group = (warp >> 2) / PARTS / SUBS;
+  const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)(sub * BN + part * COLS);
   const int64_t ld64 = P.out_stride * (int64_t)sizeof(T);
   const uint32_t ld = ld64 < (1ll << 32) ? (uint32_t)ld64 : 0u;
   float sr = 0.f, bias = 0.f, sqv[SQ];
   int64_t row0 = 0, q0 = 0;
   auto fetch = [&]() {  // of unit un
-    row0 = un.rt * tile_rows + row_off + 32 * quarter;
+    row0 = un.rt * tile_rows + row_off + sub * MMA_ROWS + 32 * quarter;
     q0 = (int64_t)un.qt * BN + part * COLS;
     const bool live = row0 + lane < P.n;
     sr = live ? __ldg(P.scales + row0 + lane) : 0.f;
@@ -237,12 +240,12 @@ __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, f
     if (!ok) s = __uint_as_float(0x7fffffffu);
     tc::fence_after();
     uint32_t v[2][W];
-    tc::ld_32x32b_x16(taddr + (uint32_t)(b * BN), v[0]);
+    tc::ld_32x32b_x16(taddr + (uint32_t)(b * BN * SUBS), v[0]);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       tc::wait_ld();
       if (i + 1 < N) {
-        tc::ld_32x32b_x16(taddr + (uint32_t)(b * BN + (i + 1) * W), v[(i + 1) & 1]);
+        tc::ld_32x32b_x16(taddr + (uint32_t)(b * BN * SUBS + (i + 1) * W), v[(i + 1) & 1]);
       } else {
         tc::fence_before();
         __syncwarp();
@@ -255,11 +258,11 @@ __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, f
   return ok;
 }
 
-template <typename T, int BN>
+template <typename T, int BN, int SUBS>
 __global__ void __launch_bounds__(MMA_THREADS, 1)
     k_scores_mma(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap cmap, ScoresParams P,
                  int q_tiles, int64_t units, Ring ring) {
-  constexpr int EW = EPILOGUE_WARPS, NB = accumulators(BN);
+  constexpr int EW = EPILOGUE_WARPS, NB = accumulators(BN, SUBS), TILE = MMA_ROWS * SUBS;
   const int S = ring.stages, STAGE = ring.stage_bytes();
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem =
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4 * column_parts(BN));  // one lane of each epilogue warp of a group
+      mbar_init(&acc_empty[b], 4 * column_parts(BN) * SUBS);  // one lane of each epilogue warp of a unit
     }
     mbar_init(&q_full, 1);
     s_failed = 0;
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
     tc::prefetch_map(&cmap);
     tc::prefetch_map(&qmap);
   }
-  if (warp == EW + 1) tc::tmem_alloc(&tmem_base, NB * BN);
+  if (warp == EW + 1) tc::tmem_alloc(&tmem_base, NB * BN * SUBS);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -304,13 +307,13 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
         for (int j = 0; j < chunks; ++j) tc::tma_load_2d(smem + S * STAGE + j * BN * 128, &qmap, 128 * j, 0, &q_full);
       }
       for (Units un(blockIdx.x, gridDim.x, q_tiles); un.u < units && ok; un.next()) {
-        const int row0 = (int)(un.rt * MMA_ROWS), q0 = un.qt * BN;
+        const int row0 = (int)(un.rt * TILE), q0 = un.qt * BN;
         for (int j = 0; j < chunks; ++j, ++filled) {
           if (filled >= S && !mbar_wait(&empty[s], ph ^ 1u, &g_error, ERR_TIMEOUT_EMPTY)) { ok = false; break; }
           mbar_arrive_expect_tx(&full[s], STAGE);  // out-of-range rows and columns arrive as zeros
           unsigned char* dst = smem + s * STAGE;
           tc::tma_load_2d(dst, &cmap, 128 * j, row0, &full[s]);
-          if (!ring.resident) tc::tma_load_2d(dst + MMA_ROWS * 128, &qmap, 128 * j, q0, &full[s]);
+          if (!ring.resident) tc::tma_load_2d(dst + TILE * 128, &qmap, 128 * j, q0, &full[s]);
           if (++s == S) { s = 0; ph ^= 1u; }
         }
       }
@@ -324,7 +327,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
     const uint32_t sbase = smem_u32(smem);
     // the chunk's queries: beside its rows in the stage, or chunk by chunk behind the ring
     const uint64_t dA = tc::sdesc_k_sw128(sbase),
-                   dB = tc::sdesc_k_sw128(sbase + (ring.resident ? S * STAGE : MMA_ROWS * 128));
+                   dB = tc::sdesc_k_sw128(sbase + (ring.resident ? S * STAGE : TILE * 128));
     const int tail = (P.d - (chunks - 1) * 128 + 31) >> 5;  // K steps of 32 in the last chunk
     int s = 0, it = 0;
     uint32_t ph = 0;
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
         break;
       }
       tc::fence_after();
-      const uint32_t acc = tmem + (uint32_t)(b * BN);
+      const uint32_t acc = tmem + (uint32_t)(b * BN * SUBS);
       for (int j = 0; j < chunks; ++j) {
         if (!__all_sync(FULL_MASK, mbar_wait(&full[s], ph, &g_error, ERR_TIMEOUT_FULL))) { ok = false; break; }
         tc::fence_after();
@@ -346,8 +349,12 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
           const uint64_t q = dB + ((uint32_t)(ring.resident ? j * BN * 128 : s * STAGE) >> 4);
           const int steps = j + 1 < chunks ? 4 : tail;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // 32 bytes of K further: 2 units of 16 bytes
-            if (k < steps) tc::mma_s8_ss(acc, a + 2 * k, q + 2 * k, idesc, (j | k) != 0 ? 1u : 0u);
+          for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // 32 bytes of K further: 2 units of 16 bytes
+              if (k < steps)
+                tc::mma_s8_ss(acc + (uint32_t)(sub * BN), a + sub * (MMA_ROWS * 128 >> 4) + 2 * k, q + 2 * k, idesc,
+                              (j | k) != 0 ? 1u : 0u);
           tc::commit(&empty[s]);
         }
         __syncwarp();
@@ -358,14 +365,14 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
     }
     if (!ok && lane == 0) s_failed = 1;
   } else {
-    const bool ok = epilogue<T, BN>(P, tmem, s_sq[warp], Units(blockIdx.x, gridDim.x, q_tiles), units, MMA_ROWS, 0,
-                                      acc_full, [&](int b) { mbar_arrive(&acc_empty[b]); });
+    const bool ok = epilogue<T, BN, SUBS>(P, tmem, s_sq[warp], Units(blockIdx.x, gridDim.x, q_tiles), units, TILE, 0,
+                                          acc_full, [&](int b) { mbar_arrive(&acc_empty[b]); });
     if (!ok && lane == 0) s_failed = 1;
   }
   tc::fence_before();
   __syncthreads();
   if (s_failed) grace_period();  // copies and MMAs of the failed waits end before the memory is freed
-  if (warp == EW + 1) tc::tmem_dealloc(tmem, NB * BN);
+  if (warp == EW + 1) tc::tmem_dealloc(tmem, NB * BN * SUBS);
 }
 
 // The same for many queries with a CTA pair a unit of 256 rows x 256 queries: each
@@ -488,7 +495,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
       if (!ok && lane == 0) s_failed = 1;
     }
   } else {
-    const bool ok = epilogue<T, PAIR_BN>(P, tmem, s_sq[warp], Units(first, step, q_tiles), units, 2 * MMA_ROWS,
+    const bool ok = epilogue<T, PAIR_BN, 1>(P, tmem, s_sq[warp], Units(first, step, q_tiles), units, 2 * MMA_ROWS,
                                       (int)rank * MMA_ROWS, acc_full,
                                       [&](int b) { tc::mbar_arrive_remote(lead_acc_empty + 8u * (uint32_t)b); });
     if (!ok && lane == 0) s_failed = 1;
@@ -532,20 +539,30 @@ static int sm_count() {
   return n;
 }
 
-template <typename T, int BN>
-static int launch_mma(const ScoresParams& P, cudaStream_t st) {
+template <typename T, int BN, int SUBS>
+static int launch_mma_units(const ScoresParams& P, cudaStream_t st) {
+  constexpr int rows = MMA_ROWS * SUBS;
   CUtensorMap qmap, cmap;
-  if (!code_map(&qmap, P.q, P.nq, P.d, P.q_stride, BN) || !code_map(&cmap, P.codes, P.n, P.d, P.code_stride, MMA_ROWS))
+  if (!code_map(&qmap, P.q, P.nq, P.d, P.q_stride, BN) || !code_map(&cmap, P.codes, P.n, P.d, P.code_stride, rows))
     return bad("int8_scores: cuTensorMapEncodeTiled refused the code rows");
   constexpr int smem = RING_BYTES + 1024;
   static SmemOptIn opt_in;
-  const int rc = check(opt_in.ensure(reinterpret_cast<const void*>(k_scores_mma<T, BN>), smem), "int8_scores shared memory");
+  const int rc = check(opt_in.ensure(reinterpret_cast<const void*>(k_scores_mma<T, BN, SUBS>), smem),
+                       "int8_scores shared memory");
   if (rc) return rc;
   const int q_tiles = (int)((P.nq + BN - 1) / BN);
-  const int64_t units = (P.n + MMA_ROWS - 1) / MMA_ROWS * q_tiles, sms = sm_count();
-  k_scores_mma<T, BN><<<(unsigned)(units < sms ? units : sms), MMA_THREADS, smem, st>>>(qmap, cmap, P, q_tiles, units,
-                                                                              Ring::of(BN, (P.d + 127) / 128, q_tiles == 1 && units > 2 * sms));
+  const int64_t units = (P.n + rows - 1) / rows * q_tiles, sms = sm_count();
+  k_scores_mma<T, BN, SUBS><<<(unsigned)(units < sms ? units : sms), MMA_THREADS, smem, st>>>(
+      qmap, cmap, P, q_tiles, units, Ring::of(rows, BN, (P.d + 127) / 128, q_tiles == 1 && units > 2 * sms));
   return CIRCUIT_OK;
+}
+template <typename T, int BN>
+static int launch_mma(const ScoresParams& P, cudaStream_t st) {
+  // two tiles a unit: rows of one chunk, several units an SM
+  if constexpr (BN <= 64) {
+    if (P.d <= 128 && P.n > 4 * 2 * MMA_ROWS * (int64_t)sm_count()) return launch_mma_units<T, BN, 2>(P, st);
+  }
+  return launch_mma_units<T, BN, 1>(P, st);
 }
 
 template <typename T, int NQ>

@@ -615,3 +615,15 @@ print("captured")
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "circuit-rag_b200")
     done = subprocess.run([sys.executable, "-c", code, root], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("d", [1, 16, 33, 64, 100, 128])
+@pytest.mark.parametrize("nq", [3, 16, 30, 32, 57, 64])
+def test_scores_of_many_short_rows(nq, d):
+    """Rows of one chunk, two tiles of them at a time, the last one partial."""
+    for n in (200_001, 300_160, 152_000 + 130):
+        dtype = TYPES[(nq + d + n) % 3]
+        qc, qs = _codes(nq, d, seed=d + nq)
+        rc, rs = _codes(n, d, seed=d)
+        bias = torch.randn(n, device=DEV) if nq % 2 else None
+        _check_scores(int8_scores(qc, qs, rc, rs, bias=bias, dtype=dtype), qc, qs, rc, rs, bias, dtype)
