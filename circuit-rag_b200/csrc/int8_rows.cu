@@ -79,7 +79,7 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
   uintptr_t bits = 16 | (uintptr_t)rows | (uintptr_t)(row_stride * e) | (uintptr_t)(dim * (int64_t)e) |
                    ((uintptr_t)codes | (uintptr_t)code_stride) * e;
   if (weight && weight_dtype == dtype) bits |= (uintptr_t)weight;
-  else if (weight && !on16(weight, 0)) bits |= (uintptr_t)weight % 8 ? 2 : 4;  // fp32 beside 16-bit words
+  else if (weight && !on16(weight, 0)) bits |= (uintptr_t)weight % 8 ? 2 : 4;  // fp32 beside 16-bit words: 4 bytes a value
   if (residual)
     bits |= (uintptr_t)residual | (uintptr_t)(residual_stride * e) | (uintptr_t)summed | (uintptr_t)(summed_stride * e);
   const int bytes = (int)(bits & -bits);

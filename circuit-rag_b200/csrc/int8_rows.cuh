@@ -375,24 +375,25 @@ static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
 // Rows of narrower words than 16 bytes: neighbouring lanes on neighbouring words.
 template <typename T, int E, bool FULL>
 static void quantize_fine(const QuantizeParams& P, cudaStream_t st) {
+  constexpr int MOST = CIRCUIT_INT8_MAX_DIM / E;
   const int words = P.d / E;
-  if (P.n <= FEW_ROWS) {
-    if (words <= 128) launch_quantize<T, E, 32, 4, FULL>(P, st);
-    else if (words <= 512) launch_quantize<T, E, 32, 16, FULL>(P, st);
-    else if (words <= 1024) launch_quantize<T, E, 128, 8, FULL>(P, st);
-    else if (words <= 4096) launch_quantize<T, E, 512, 8, FULL>(P, st);
-    else if (words <= 8192) launch_quantize<T, E, 512, 16, FULL>(P, st);
-    else if constexpr (E == 1) launch_quantize<T, E, 512, 32, FULL>(P, st);
-  } else if (words <= 32) launch_quantize<T, E, 4, 8, FULL>(P, st);
+  if (P.n <= FEW_ROWS && words > 32) {
+    if (words <= 128) return launch_quantize<T, E, 32, 4, FULL>(P, st);
+    if (words > 512 && words <= 1024) return launch_quantize<T, E, 128, 8, FULL>(P, st);
+    if (words > 1024 && words <= 4096) return launch_quantize<T, E, 256, 16, FULL>(P, st);
+  }
+  if (words <= 32) launch_quantize<T, E, 4, 8, FULL>(P, st);
   else if (words <= 64) launch_quantize<T, E, 8, 8, FULL>(P, st);
   else if (words <= 128) launch_quantize<T, E, 8, 16, FULL>(P, st);
-  else if (words <= 256) launch_quantize<T, E, 16, 16, FULL>(P, st);
+  else if (words <= 256 && P.n > FEW_ROWS) launch_quantize<T, E, 16, 16, FULL>(P, st);
   else if (words <= 512) launch_quantize<T, E, 32, 16, FULL>(P, st);
   else if (words <= 1024) launch_quantize<T, E, FULL ? 128 : 32, FULL ? 8 : 32, FULL>(P, st);
   else if (words <= 2048) launch_quantize<T, E, 128, 16, FULL>(P, st);
   else if (words <= 4096) launch_quantize<T, E, 256, 16, FULL>(P, st);
-  else if (words <= 8192) launch_quantize<T, E, 512, 16, FULL>(P, st);
-  else if constexpr (E == 1) launch_quantize<T, E, 512, 32, FULL>(P, st);
+  else if constexpr (MOST > 4096) {
+    if (words <= 8192) launch_quantize<T, E, 512, 16, FULL>(P, st);
+    else if constexpr (MOST > 8192) launch_quantize<T, E, 512, 32, FULL>(P, st);
+  }
 }
 // bytes: the widest word (16, or less) that the rows are whole words of.
 template <typename T, bool FULL>
@@ -400,8 +401,9 @@ static void quantize(const QuantizeParams& P, int bytes, cudaStream_t st) {
   constexpr int V = RowType<T>::V;
   if (bytes < 16) {
     if constexpr (V == 8) {
-      if (bytes >= 4) return quantize_fine<T, 2, FULL>(P, st);
+      if (bytes >= 8) return quantize_fine<T, 4, FULL>(P, st);
     }
+    if (bytes >= 2 * (int)sizeof(T)) return quantize_fine<T, 2, FULL>(P, st);
     return quantize_fine<T, 1, FULL>(P, st);
   }
   const int vectors = P.d / V;
@@ -449,8 +451,9 @@ static void dequantize(const ReadParams& P, int bytes, cudaStream_t st) {
   const int vectors = P.d / V;
   if (bytes < 16) {
     if constexpr (V == 8) {
-      if (bytes >= 4) return read_fine<T, 2>(P, st);
+      if (bytes >= 8) return read_fine<T, 4>(P, st);
     }
+    if (bytes >= 2 * (int)sizeof(T)) return read_fine<T, 2>(P, st);
     return read_fine<T, 1>(P, st);
   }
   if (vectors <= 4) launch_read<T, V, 4, 1>(P, st);

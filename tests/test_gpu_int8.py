@@ -46,8 +46,8 @@ def _check_plain(x, codes, scales):
     assert torch.equal(scales, (a / 127).float())
 
 
-DIMS = [1, 2, 7, 16, 31, 33, 64, 128, 136, 200, 256, 384, 385, 511, 512, 513, 640, 768, 1000, 1024, 1025, 1536, 2048, 2049,
-        4096, 4100, 8191, 8192, 16384]
+DIMS = [1, 2, 6, 7, 16, 31, 33, 64, 100, 128, 130, 136, 200, 256, 384, 385, 511, 512, 513, 514, 604, 640, 768, 1000, 1024,
+        1025, 1030, 1536, 2048, 2049, 4096, 4100, 4102, 8191, 8192, 8196, 8198, 16382, 16384]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
