@@ -10,12 +10,16 @@ namespace cb {
 namespace i8 {
 
 __global__ void k_reset_slots(const void* slots, int slot64, int64_t n, int64_t capacity, float* scales) {
+  griddep_wait();
+  griddep_launch();
   const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
   if (i >= n) return;
   const int64_t s = slot_at(slots, slot64, i);
   if (s >= 0 && s < capacity) scales[s] = 0.f;
 }
 __global__ void k_claim_slots(const void* slots, int slot64, int64_t n, int64_t capacity, float* scales) {
+  griddep_wait();
+  griddep_launch();
   const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
   if (i >= n) return;
   const int64_t s = slot_at(slots, slot64, i);
@@ -89,8 +93,8 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
   P.claimed = slots && n > 1024;
   if (P.claimed) {
     const unsigned blocks = (unsigned)((n + 255) / 256);
-    k_reset_slots<<<blocks, 256, 0, st>>>(slots, P.slot64, n, capacity, scales);
-    k_claim_slots<<<blocks, 256, 0, st>>>(slots, P.slot64, n, capacity, scales);
+    launch(k_reset_slots, dim3(blocks), 256, 0, 1, st, slots, P.slot64, n, capacity, scales);
+    launch(k_claim_slots, dim3(blocks), 256, 0, 1, st, slots, P.slot64, n, capacity, scales);
   }
   const bool full = norm != CIRCUIT_NORM_NONE;
   if (dtype == CIRCUIT_F32) quantize_rows<float>(P, bytes, full, st);

@@ -167,6 +167,8 @@ __device__ __noinline__ void exact_codes(const QuantizeParams& P, const T* src, 
 // work of each row (reduction, addresses, scale) is shared by the rows of a warp.
 template <typename T, int E, int G, int NV, bool FULL>
 __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_constant__ QuantizeParams P) {
+  griddep_wait();
+  griddep_launch();
   const int lane = threadIdx.x % G;
   const int64_t row = (int64_t)blockIdx.x * (row_threads(G) / G) + threadIdx.x / G;
   const bool live = row < P.n;
@@ -319,6 +321,8 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
 // id below 0 is an empty place (zeros), one past the store a mistake (NaN).
 template <typename T, int E, int G, int NV>
 __global__ void __launch_bounds__(256) k_dequantize_rows(const __grid_constant__ ReadParams P) {
+  griddep_wait();
+  griddep_launch();
   const int lane = threadIdx.x % G;
   const int64_t i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   if (i >= P.n) return;
@@ -370,7 +374,7 @@ constexpr int64_t FEW_ROWS = 148 * 8, FEW_LONG_ROWS = 148 * 2;
 template <typename T, int E, int G, int NV, bool FULL>
 static void launch_quantize(const QuantizeParams& P, cudaStream_t st) {
   constexpr int threads = row_threads(G), rows = threads / G;
-  k_quantize_rows<T, E, G, NV, FULL><<<(unsigned)((P.n + rows - 1) / rows), threads, 0, st>>>(P);
+  launch(k_quantize_rows<T, E, G, NV, FULL>, dim3((unsigned)((P.n + rows - 1) / rows)), threads, 0, 1, st, P);
 }
 // Rows of narrower words than 16 bytes: neighbouring lanes on neighbouring words.
 template <typename T, int E, bool FULL>
@@ -434,7 +438,7 @@ static void quantize(const QuantizeParams& P, int bytes, cudaStream_t st) {
 template <typename T, int E, int G, int NV>
 static void launch_read(const ReadParams& P, cudaStream_t st) {
   constexpr int rows = 256 / G;
-  k_dequantize_rows<T, E, G, NV><<<(unsigned)((P.n + rows - 1) / rows), 256, 0, st>>>(P);
+  launch(k_dequantize_rows<T, E, G, NV>, dim3((unsigned)((P.n + rows - 1) / rows)), 256, 0, 1, st, P);
 }
 template <typename T, int E>
 static void read_fine(const ReadParams& P, cudaStream_t st) {

@@ -34,6 +34,8 @@ __device__ __forceinline__ float result(int acc, float sq, float sr, float bias)
 // holds does not count).
 template <typename T, int NQ>
 __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
+  griddep_wait();
+  griddep_launch();
   extern __shared__ __align__(16) int8_t s_q[];
   const int chunks = (P.d + 15) >> 4;
   const int64_t q0 = (int64_t)blockIdx.y * NQ;
@@ -295,6 +297,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = tmem_base;
+  griddep_wait();  // codes and scales may come from the kernel before
+  griddep_launch();
 
   if (warp == EW) {
     if (lane == 0) {
@@ -424,6 +428,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 1)
   tc::cluster_sync();  // barriers and the pair's TMEM exist before any remote access
   tc::fence_after();
   const uint32_t tmem = tmem_base;
+  griddep_wait();  // codes and scales may come from the kernel before
+  griddep_launch();
   const uint32_t lead_full = tc::mapa_shared(smem_u32(&full[0]), 0);
   const uint32_t lead_acc_empty = tc::mapa_shared(smem_u32(&acc_empty[0]), 0);
 
@@ -552,9 +558,10 @@ static int launch_mma_units(const ScoresParams& P, cudaStream_t st) {
   if (rc) return rc;
   const int q_tiles = (int)((P.nq + BN - 1) / BN);
   const int64_t units = (P.n + rows - 1) / rows * q_tiles, sms = sm_count();
-  k_scores_mma<T, BN, SUBS><<<(unsigned)(units < sms ? units : sms), MMA_THREADS, smem, st>>>(
-      qmap, cmap, P, q_tiles, units, Ring::of(rows, BN, (P.d + 127) / 128, q_tiles == 1 && units > 2 * sms));
-  return CIRCUIT_OK;
+  return check(launch(k_scores_mma<T, BN, SUBS>, dim3((unsigned)(units < sms ? units : sms)), MMA_THREADS, smem, 1, st,
+                      qmap, cmap, P, q_tiles, units,
+                      Ring::of(rows, BN, (P.d + 127) / 128, q_tiles == 1 && units > 2 * sms)),
+               "int8_scores launch");
 }
 template <typename T, int BN>
 static int launch_mma(const ScoresParams& P, cudaStream_t st) {
@@ -571,8 +578,7 @@ static int launch_rows(const ScoresParams& P, cudaStream_t st) {
   const int smem = NQ * ((P.d + 15) / 16) * 16;
   const int64_t blocks = (P.n + 31) / 32;
   const dim3 grid((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), (unsigned)((P.nq + NQ - 1) / NQ));
-  k_scores_rows<T, NQ><<<grid, 256, smem, st>>>(P);
-  return CIRCUIT_OK;
+  return check(launch(k_scores_rows<T, NQ>, grid, 256, smem, 1, st, P), "int8_scores launch");
 }
 template <typename T>
 static int launch_pair(const ScoresParams& P, cudaStream_t st) {
@@ -586,21 +592,12 @@ static int launch_pair(const ScoresParams& P, cudaStream_t st) {
   if (rc) return rc;
   const int q_tiles = (int)((P.nq + PAIR_BN - 1) / PAIR_BN);
   const int64_t units = (P.n + 2 * MMA_ROWS - 1) / (2 * MMA_ROWS) * q_tiles, pairs = sm_count() / 2;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = 2;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(2 * (units < pairs ? units : pairs)));
-  cfg.blockDim = dim3(MMA_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &cluster;
-  cfg.numAttrs = 1;
   // short sums are bound by the results' way out, which less in flight disturbs less (200,000 x 100 fp16, 558 queries: 4
   // stages 63 us, 6 stages 69; 1,024 x 40,000 x 768: 34 and 31)
   const int stages = P.d <= 512 ? 4 : PAIR_STAGES;
-  return check(cudaLaunchKernelEx(&cfg, k_scores_pair<T>, qmap, cmap, P, q_tiles, units, stages), "int8_scores launch");
+  return check(launch(k_scores_pair<T>, dim3((unsigned)(2 * (units < pairs ? units : pairs))), MMA_THREADS, smem, 2, st, qmap,
+                      cmap, P, q_tiles, units, stages),
+               "int8_scores launch");
 }
 
 template <typename T>

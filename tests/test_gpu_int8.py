@@ -627,3 +627,33 @@ def test_scores_of_many_short_rows(nq, d):
         rc, rs = _codes(n, d, seed=d)
         bias = torch.randn(n, device=DEV) if nq % 2 else None
         _check_scores(int8_scores(qc, qs, rc, rs, bias=bias, dtype=dtype), qc, qs, rc, rs, bias, dtype)
+
+
+@pytest.mark.parametrize("nq,n", [(1, 3000), (2, 60000), (40, 9000), (300, 9000), (1000, 40000)])
+def test_chains_over_the_same_buffers(nq, n):
+    """Kernels of a chain start early and wait for the one before: the same buffers are written and read again and
+    again without a synchronisation, and every step's results are those of its own inputs."""
+    d = 256
+    rc, rs = _codes(n, d, seed=n)
+    inputs = [_rows(nq, d, torch.bfloat16, seed) for seed in range(6)]
+    x = torch.empty_like(inputs[0])
+    qc, qs = torch.empty(nq, d, dtype=torch.int8, device=DEV), torch.empty(nq, device=DEV)
+    out, back = torch.empty(nq, n, device=DEV), torch.empty(nq, d, device=DEV)
+    slots = torch.randperm(n, device=DEV)[:nq]
+    kept = []
+    torch.cuda.synchronize()
+    for step in range(24):
+        x.copy_(inputs[step % 6])
+        quantize_rows(x, out=(qc, qs))
+        dequantize_rows(qc, qs, out=back)
+        int8_scores(qc, qs, rc, rs, out=out)
+        quantize_rows(x, slots=slots, out=(rc, rs))  # changes rows for the next step
+        kept.append((qc.clone(), qs.clone(), back.clone(), out[:, ::97].clone(), rc[slots].clone()))
+    rc, rs = _codes(n, d, seed=n)
+    cols = torch.arange(0, n, 97, device=DEV)
+    for step, (c, s, b, got, written) in enumerate(kept):
+        _check_plain(inputs[step % 6], c, s)
+        assert torch.equal(b, c.float() * s[:, None])
+        _check_scores(got, c, s, rc[cols], rs[cols], None, torch.float32)
+        rc[slots], rs[slots] = c, s
+        assert torch.equal(written, c)
