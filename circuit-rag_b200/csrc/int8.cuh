@@ -113,7 +113,9 @@ struct Vec {
 // Launches a kernel that may start while the one before it on the stream still runs:
 // each of these kernels first waits for that one's completion (griddep_wait, before
 // any access to memory) and only then lets the next one start early, so that no more
-// than two of a chain overlap.  What is saved is the launch and the set-up, one to
+// than two of a chain overlap.  They read global memory by ordinary loads: a load by the
+// non-coherent path asks for data that no one writes while the kernel lives, and the
+// one before still writes when these start.  What is saved is the launch and the set-up, one to
 // two microseconds a kernel (a pass of one query against 2M rows: 128 -> 120 us).
 template <typename... Params, typename... Args>
 inline cudaError_t launch(void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster, cudaStream_t st,

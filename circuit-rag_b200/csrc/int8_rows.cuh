@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(256) k_dequantize_rows(const __grid_constant__
   if (i >= P.n) return;
   const int64_t id = P.ids ? slot_at(P.ids, P.id64, i) : i;
   const bool known = id >= 0 && id < P.rows;
-  const float scale = known ? __ldg(P.scales + id) : id < 0 ? 0.f : __uint_as_float(0x7fffffffu);
+  const float scale = known ? P.scales[id] : id < 0 ? 0.f : __uint_as_float(0x7fffffffu);
   const int8_t* in = P.codes + (known ? id : 0) * P.code_stride;
   T* out = reinterpret_cast<T*>(P.out) + i * P.out_stride;
   const int d = P.d, dk = known ? P.d : 0;
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(256) k_dequantize_rows(const __grid_constant__
 #pragma unroll
       for (int j = 0; j < (E + 3) / 4; ++j) w[k][j] = 0;
       if (c < dk) {
-        const typename Word<E>::type word = __ldg(reinterpret_cast<const typename Word<E>::type*>(in + c));
+        const typename Word<E>::type word = *reinterpret_cast<const typename Word<E>::type*>(in + c);
         memcpy(w[k], &word, E);
       }
     }

@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
 #pragma unroll
     for (int q = 0; q < NQ; ++q) acc[q] = 0;
     for (int c = sub; c < chunks; c += 8) {
-      const int4 b = __ldg(r + c);
+      const int4 b = r[c];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
         const int4 a = reinterpret_cast<const int4*>(s_q)[q * chunks + c];
@@ -68,8 +68,7 @@ __global__ void __launch_bounds__(256) k_scores_rows(ScoresParams P) {
       for (int o = 4; o > 0; o >>= 1) acc[q] += __shfl_xor_sync(FULL_MASK, acc[q], o);
       if (live && sub == (q & 7) && q0 + q < P.nq)
         reinterpret_cast<T*>(P.out)[(q0 + q) * P.out_stride + row] =
-            RowType<T>::put(result(acc[q], __ldg(P.q_scales + q0 + q), __ldg(P.scales + row),
-                                   P.bias ? __ldg(P.bias + row) : 0.f));
+            RowType<T>::put(result(acc[q], P.q_scales[q0 + q], P.scales[row], P.bias ? P.bias[row] : 0.f));
     }
   }
 }
@@ -214,11 +213,11 @@ __device__ __forceinline__ bool epilogue(const ScoresParams& P, uint32_t tmem, f
     row0 = un.rt * tile_rows + row_off + sub * MMA_ROWS + 32 * quarter;
     q0 = (int64_t)un.qt * BN + part * COLS;
     const bool live = row0 + lane < P.n;
-    sr = live ? __ldg(P.scales + row0 + lane) : 0.f;
-    bias = live && P.bias ? __ldg(P.bias + row0 + lane) : 0.f;
+    sr = live ? P.scales[row0 + lane] : 0.f;
+    bias = live && P.bias ? P.bias[row0 + lane] : 0.f;
 #pragma unroll
     for (int i = 0; i < SQ; ++i)
-      sqv[i] = 32 * i + lane < COLS && q0 + 32 * i + lane < P.nq ? __ldg(P.q_scales + q0 + 32 * i + lane) : 0.f;
+      sqv[i] = 32 * i + lane < COLS && q0 + 32 * i + lane < P.nq ? P.q_scales[q0 + 32 * i + lane] : 0.f;
   };
   for (int i = 0; i < group; ++i) un.next();
   if (un.u < units) fetch();
