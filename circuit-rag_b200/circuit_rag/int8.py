@@ -100,7 +100,8 @@ class Int8Rows:
 
     def _buffers(self, n: int):
         codes = torch.zeros((n, (self.dim + 15) // 16 * 16), dtype=torch.int8, device=self.device)
-        return codes, torch.full((n,), float("nan"), dtype=torch.float32, device=self.device)
+        # one scale more than places: what is meant for no place goes there
+        return codes, torch.full((n + 1,), float("nan"), dtype=torch.float32, device=self.device)
 
     def __len__(self) -> int:
         return self._len
@@ -135,8 +136,12 @@ class Int8Rows:
         return range(first, need)
 
     def remove(self, slots: torch.Tensor) -> None:
-        """Empties the places ``slots`` (all inside the store)."""
-        self.scales[slots.to(device=self.device, dtype=torch.int64)] = float("nan")
+        """Empties the places ``slots`` (whole numbers, any shape).  A slot outside the store changes nothing."""
+        if not isinstance(slots, torch.Tensor) or slots.dtype == torch.bool or slots.is_floating_point() or slots.is_complex():
+            raise ValueError("slots must be a tensor of whole numbers")
+        at = slots.to(device=self.device, dtype=torch.int64).reshape(-1)
+        at = at.masked_fill((at < 0) | (at >= self._len), self._codes.shape[0])
+        self._scales.index_fill_(0, at, float("nan"))
 
     def read(self, ids: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The rows at ``ids`` (any shape, as a search returns them; -1 gives zeros)."""
