@@ -112,7 +112,8 @@ int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const f
   if (n < 0 || n > 0x7fffffffLL || rows < 0) return bad("dequantize_rows: bad sizes");
   if (ids && id_bytes != 4 && id_bytes != 8) return bad("dequantize_rows: ids must be int32 or int64");
   if (n == 0) return CIRCUIT_OK;
-  if (!codes || !scales || !out) return bad("dequantize_rows: null pointer");
+  // a store without rows has no memory either: every id is then an empty place or past the end
+  if ((rows > 0 && (!codes || !scales)) || !out) return bad("dequantize_rows: null pointer");
   if (!ids && rows < n) return bad("dequantize_rows: more rows asked for than there are");
   if (code_stride < dim || out_stride < dim) return bad("dequantize_rows: a row stride is smaller than dim");
   if ((uintptr_t)out % e || (uintptr_t)scales % 4 || (ids && (uintptr_t)ids % id_bytes))

@@ -117,7 +117,8 @@ int circuit_op_quantize_rows(const void* rows, int dtype, int64_t n, int dim, in
                              void* stream);
 
 /* out[i] = codes[id] * scales[id] for id = ids[i] (int32 or int64), or i when ids == NULL, rounded once to dtype.
- * A negative id is an empty place and gives zeros, an id >= rows gives NaN. */
+ * A negative id is an empty place and gives zeros, an id >= rows gives NaN.  With rows == 0 codes and scales may be
+ * NULL. */
 int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const float* scales, int64_t rows, int dim,
                                const void* ids, int id_bytes, int64_t n, void* out, int dtype, int64_t out_stride,
                                void* stream);

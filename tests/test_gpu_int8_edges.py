@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from circuit_rag import Int8Rows
+from circuit_rag import Int8Rows, dequantize_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,18 @@ def test_remove_skips_what_is_outside_the_store():
     graph.replay()
     torch.cuda.synchronize()
     assert _held(store) == [0, 1, 3, 5, 6]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [1, 8, 33, 384, 1000, 5000])
+def test_read_of_a_store_without_rows(d, dtype):
+    store = Int8Rows(0, d, DEV)
+    ids = store.search(_rows(3, d), 4)[1]
+    assert (ids == -1).all()
+    assert torch.equal(store.read(ids, dtype=dtype), torch.zeros(3, 4, d, dtype=dtype, device=DEV))
+    for n in (5, 2000):  # few rows and many
+        ids = torch.randint(-3, 4, (n,), device=DEV)
+        got = store.read(ids, dtype=dtype)
+        assert (got[ids < 0] == 0).all() and got[ids >= 0].isnan().all()
+    assert store.read(ids[:0]).shape == (0, d)
+    assert dequantize_rows(store.codes, store.scales).shape == (0, d)
