@@ -81,6 +81,13 @@ def int8_scores(query_codes: torch.Tensor, query_scales: torch.Tensor, codes: to
     return _bind().scores(query_codes, query_scales, codes, scales, bias, dtype, out)
 
 
+def check_products(device=None) -> None:
+    """Waits for the current stream of ``device`` and raises NativeLibraryError if a product on it has given up a
+    bounded wait since the last call: int8_scores writes NaN for what it could not compute."""
+    with torch.cuda.device(device):
+        _native.check(_native.lib().circuit_op_int8_status(torch.cuda.current_stream().cuda_stream), "int8_scores")
+
+
 class Int8Rows:
     """A store of 8-bit rows on one device: places that hold a row or none.
 
@@ -155,7 +162,9 @@ class Int8Rows:
 
     def search(self, queries: torch.Tensor, k: int = 10, normalize: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
         """The k best places of each query [nq, dim] by its product with the stored rows: (scores [nq, k] descending,
-        ids [nq, k] int32), ties to the lower place, score -inf and id -1 where there are fewer rows; 1 <= k <= 256."""
+        ids [nq, k] int32), ties to the lower place, score -inf and id -1 where there are fewer rows; 1 <= k <= 256.
+        A query with an infinity or NaN has no results.  A place whose row's product is NaN all the same (the kernel
+        gave up a wait, see check_products, or left the range of float32) comes first, with score NaN."""
         return self.search_codes(*quantize_rows(queries, normalize=normalize), k=k)
 
     # scores of a block of rows that are ranked at a time
@@ -172,13 +181,14 @@ class Int8Rows:
         for a in range(0, n if nq else 0, block):
             b = min(n, a + block)
             s = int8_scores(query_codes, query_scales, self._codes[a:b, :self.dim], self._scales[a:b])
-            # one whole number a score: the order of floats in the upper half, the lower place first in the lower half
+            # one whole number a score: the order of floats (NaN above all, as the kernel writes it) in the upper half,
+            # the lower place first in the lower half
             bits = s.view(torch.int32).to(torch.int64)
             bits ^= (bits >> 31) & 0x7FFFFFFF
             key = (bits << 32) + (0xFFFFFFFF - torch.arange(a, b, device=self.device))
-            key.masked_fill_(s.isnan(), none)
+            key.masked_fill_(self._scales[a:b].isnan(), none)
             best = torch.cat([best, key], 1).topk(k, dim=1).values
-        empty = best == none
+        empty = (best == none) | query_scales.isnan()[:, None]
         bits = best >> 32
         bits ^= (bits >> 31) & 0x7FFFFFFF
         scores = bits.to(torch.int32).view(torch.float32).masked_fill_(empty, float("-inf"))

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from circuit_rag.hierarchy.build import build_circuit_index
-from circuit_rag.int8 import Int8Rows, rms_norm_quantize
+from circuit_rag.int8 import Int8Rows, check_products, rms_norm_quantize
 from circuit_rag.search import circuit_search
 
 
@@ -108,8 +108,12 @@ class CircuitRAG:
             scores, ids = self._search_rows(q.to(self.store.device)[None], k, feedback or [])
         else:
             scores, ids, _ = circuit_search(q, self.index, k=k)
+        scores, ids = scores.tolist(), ids.tolist()
+        if self.rows == "int8" and any(s != s for s in scores):  # not a missing document: a product was not computed
+            check_products(self.store.device)
+            raise RuntimeError("a product of the query and a document is not a number")
         return [SearchResult(id=int(i), score=float(s), text=self.texts[int(i)], metadata=self.metadatas[int(i)])
-                for s, i in zip(scores.tolist(), ids.tolist()) if i >= 0]
+                for s, i in zip(scores, ids) if i >= 0]
 
     def _search_rows(self, q: torch.Tensor, k: int, feedback: List[int]):
         if any(not 0 <= i < len(self.texts) for i in feedback):

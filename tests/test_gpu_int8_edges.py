@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from circuit_rag import Int8Rows, dequantize_rows
+from circuit_rag import Int8Rows, dequantize_rows, int8, int8_scores, quantize_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,28 @@ def test_read_of_a_store_without_rows(d, dtype):
         assert (got[ids < 0] == 0).all() and got[ids >= 0].isnan().all()
     assert store.read(ids[:0]).shape == (0, d)
     assert dequantize_rows(store.codes, store.scales).shape == (0, d)
+
+
+@pytest.mark.parametrize("nq", [1, 3, 20, 200])
+@pytest.mark.parametrize("n", [300, 50000])
+def test_a_product_without_a_number_comes_first(n, nq):
+    """Empty places and queries without a number have no results; any other NaN (here infinity times a row of zeros) shows."""
+    store = Int8Rows(0, 32, DEV)
+    x = _rows(n, 32, 1)
+    x[7] = 0
+    x[9] = float("nan")
+    store.append(x)
+    store.remove(torch.tensor([11], device=DEV))
+    qc, qs = quantize_rows(_rows(nq, 32, 2))
+    qs[nq // 2] = float("inf")
+    scores, ids = store.search_codes(qc, qs, k=2)
+    assert ids[nq // 2, 0] == 7 and scores[nq // 2, 0].isnan()
+    rest = torch.arange(nq, device=DEV) != nq // 2
+    assert scores[rest].isfinite().all()
+    qs[nq // 2] = float("nan")
+    scores, ids = store.search_codes(qc, qs, k=2)
+    assert (ids[nq // 2] == -1).all() and (scores[nq // 2] == -float("inf")).all() and (ids[rest] >= 0).all()
+    for k in range(0, n, 9973):  # the kernels' NaN is the one that ranks above every number
+        assert (int8_scores(qc, qs, store.codes, store.scales)[nq // 2, k].view(torch.int32) == 0x7FFFFFFF).all()
+    int8.check_products()
+    int8.check_products(DEV)

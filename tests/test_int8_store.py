@@ -1,10 +1,12 @@
 """The store of 8-bit rows on the host: what its calls do before and after the kernels, on CPU buffers."""
+import contextlib
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from circuit_rag import Int8Rows
+from circuit_rag import CircuitRAG, Int8Rows, _native, int8
 
 
 def _host_store(places, dim=8):
@@ -54,3 +56,61 @@ def test_remove_refuses_what_is_no_place(slots):
     with pytest.raises(ValueError):
         store.remove(slots)
     assert _held(store) == [0, 1, 2]
+
+
+def _search(store, products, query_scales, k, monkeypatch):
+    """search_codes with given products, as if the kernel had written them."""
+    def fake(qc, qs, codes, scales, **kw):
+        a = (codes.data_ptr() - store._codes.data_ptr()) // store._codes.shape[1]
+        return products[:, a:a + codes.shape[0]].clone()
+
+    monkeypatch.setattr(int8, "int8_scores", fake)
+    return store.search_codes(torch.zeros(products.shape[0], store.dim, dtype=torch.int8), query_scales, k=k)
+
+
+def test_a_product_that_gave_up_is_not_an_empty_place(monkeypatch):
+    """NaN at a place with a row is a failure that shows; NaN at an empty place, or of a query without a number, is
+    no result."""
+    nan, inf = float("nan"), float("inf")
+    store = _host_store(4)
+    store.remove(torch.tensor([1]))
+    products = torch.tensor([[3.0, nan, 5.0, nan], [1.0, nan, -inf, 2.0], [nan, nan, nan, nan], [nan, nan, nan, nan]])
+    scores, ids = _search(store, products, torch.tensor([1.0, 1.0, nan, 1.0]), 4, monkeypatch)
+    assert ids.tolist() == [[3, 2, 0, -1], [3, 0, 2, -1], [-1] * 4, [0, 2, 3, -1]]
+    assert scores[0, 0].isnan() and scores[0, 1:].tolist() == [5.0, 3.0, -inf]
+    assert scores[1].tolist() == [2.0, 1.0, -inf, -inf]
+    assert scores[2].tolist() == [-inf] * 4
+    assert scores[3, :3].isnan().all() and scores[3, 3] == -inf
+
+
+def test_status_reaches_python(monkeypatch):
+    class Lib:
+        calls = []
+
+        def circuit_op_int8_status(self, stream):
+            self.calls.append(stream)
+            return -4 if len(self.calls) > 1 else 0
+
+    fake = Lib()
+    monkeypatch.setattr(_native, "lib", lambda: fake)
+    monkeypatch.setattr(_native, "last_error", lambda: "a bounded wait gave up")
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": 7})())
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    int8.check_products()
+    with pytest.raises(_native.NativeLibraryError, match="gave up"):
+        int8.check_products()
+    assert fake.calls == [7, 7]
+
+
+def test_rag_reports_a_product_that_gave_up(monkeypatch):
+    rag = CircuitRAG(device="cpu", embed_fn=lambda texts: np.ones((len(texts), 8), np.float32), rows="int8")
+    rag.texts, rag.metadatas, rag.store = list("abcde"), [{}] * 5, _host_store(5)
+    results = [(torch.tensor([2.0, 1.0, -math.inf]), torch.tensor([4, 0, -1], dtype=torch.int32))]
+    monkeypatch.setattr(rag, "_search_rows", lambda q, k, feedback: results[-1])
+    checked = []
+    monkeypatch.setattr("circuit_rag.rag.check_products", lambda device: checked.append(device))
+    assert [r.id for r in rag.search("q", k=3)] == [4, 0] and checked == []
+    results.append((torch.tensor([math.nan, 1.0, -math.inf]), torch.tensor([3, 0, -1], dtype=torch.int32)))
+    with pytest.raises(RuntimeError):
+        rag.search("q", k=3)
+    assert checked == [rag.store.device]
