@@ -104,6 +104,7 @@ class Int8Rows:
         self.dim = int(dim)
         self._len = int(places)
         self._codes, self._scales = self._buffers(self._len)
+        self.device = self._codes.device  # with its index: the current device may change
 
     def _buffers(self, n: int):
         codes = torch.zeros((n, (self.dim + 15) // 16 * 16), dtype=torch.int8, device=self.device)

@@ -81,3 +81,10 @@ def test_a_product_without_a_number_comes_first(n, nq):
         assert (int8_scores(qc, qs, store.codes, store.scales)[nq // 2, k].view(torch.int32) == 0x7FFFFFFF).all()
     int8.check_products()
     int8.check_products(DEV)
+
+
+def test_places_stay_on_their_device():
+    """A device without an index is the current one when the store is made, not when it grows or searches."""
+    store = Int8Rows(2, 16, "cuda")
+    assert store.device == torch.device("cuda", torch.cuda.current_device()) == store.codes.device
+    assert Int8Rows(2, 16).device == store.device

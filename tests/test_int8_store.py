@@ -114,3 +114,27 @@ def test_rag_reports_a_product_that_gave_up(monkeypatch):
     with pytest.raises(RuntimeError):
         rag.search("q", k=3)
     assert checked == [rag.store.device]
+
+
+def test_a_growing_store_stays_on_its_device(monkeypatch):
+    """A device without an index means the current one: it is looked up once, when the store is made."""
+    asked, current = [], [torch.device("cuda", 3)]
+    host = {name: getattr(torch, name) for name in ("zeros", "full", "empty")}
+
+    class Placed:  # a tensor that says where it would lie
+        def __init__(self, tensor, device):
+            self.tensor, self.device, self.shape = tensor, device, tensor.shape
+
+    def make(name):
+        def made(*args, device=None, **kw):
+            device = torch.device(device)
+            asked.append(device if device.index is not None else current[0])
+            return Placed(host[name](*args, **kw), asked[-1])
+        return made
+
+    for name in host:
+        monkeypatch.setattr(torch, name, make(name))
+    store = Int8Rows(2, 8, "cuda")
+    current[0] = torch.device("cuda", 0)  # another device is current by now
+    codes, scales = store._buffers(9)
+    assert store.device == torch.device("cuda", 3) and set(asked) == {store.device}
