@@ -88,12 +88,21 @@ def check_products(device=None) -> None:
         _native.check(_native.lib().circuit_op_int8_status(torch.cuda.current_stream().cuda_stream), "int8_scores")
 
 
+def _stream(device: torch.device) -> int:
+    """The current stream of a device, as a plain number."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 class Int8Rows:
     """A store of 8-bit rows on one device: places that hold a row or none.
 
     ``codes`` [len, dim] and ``scales`` [len] are what int8_scores and dequantize_rows take; a place without a row has
     scale NaN, reads as NaN and is never a search result.  Calls on one store are ordered by their streams: writing
-    places while another stream reads them is the caller's to order."""
+    places while another stream reads them is the caller's to order.  An append that outgrows the buffers moves every
+    place to new ones, so to later calls on other streams it counts as writing every place; calls that are under way
+    elsewhere still have the old buffers, which are not used again before these calls are done.  ``codes`` and
+    ``scales`` taken before an append, and calls captured into a graph before it, see the places as they were then:
+    take and capture them again."""
 
     def __init__(self, places: int, dim: int, device="cuda"):
         if not 1 <= dim <= _native.CIRCUIT_INT8_MAX_DIM or not 0 <= places < 2 ** 31:
@@ -103,23 +112,36 @@ class Int8Rows:
             raise RuntimeError("8-bit rows live on a CUDA device (no CPU path)")
         self.dim = int(dim)
         self._len = int(places)
+        self._in_graph, self._captured = False, []  # a captured call uses the buffers; older buffers of such calls
         self._codes, self._scales = self._buffers(self._len)
         self.device = self._codes.device  # with its index: the current device may change
+        self._made_on = _stream(self.device)
 
     def _buffers(self, n: int):
         codes = torch.zeros((n, (self.dim + 15) // 16 * 16), dtype=torch.int8, device=self.device)
         # one scale more than places: what is meant for no place goes there
         return codes, torch.full((n + 1,), float("nan"), dtype=torch.float32, device=self.device)
 
+    def _use(self) -> None:
+        """The current stream uses the buffers: their memory is kept for it when a growing store drops them."""
+        if _stream(self.device) != self._made_on:
+            stream = torch.cuda.current_stream(self.device)
+            self._codes.record_stream(stream)
+            self._scales.record_stream(stream)
+        if torch.cuda.is_current_stream_capturing():
+            self._in_graph = True
+
     def __len__(self) -> int:
         return self._len
 
     @property
     def codes(self) -> torch.Tensor:
+        self._use()
         return self._codes[:self._len, :self.dim]
 
     @property
     def scales(self) -> torch.Tensor:
+        self._use()
         return self._scales[:self._len]
 
     def write(self, rows: torch.Tensor, slots: torch.Tensor, normalize: bool = False) -> None:
@@ -134,11 +156,17 @@ class Int8Rows:
         first, need = self._len, self._len + rows.shape[0]
         if need >= 2 ** 31:
             raise ValueError("a store holds less than 2^31 rows")
+        self._use()
         if need > self._codes.shape[0]:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a store does not grow inside a graph: each replay would copy the old rows")
+            if self._in_graph:
+                self._captured.append((self._codes, self._scales))
+                self._in_graph = False
             codes, scales = self._buffers(max(need, 2 * self._codes.shape[0]))
             codes[:first].copy_(self._codes[:first])
             scales[:first].copy_(self._scales[:first])
-            self._codes, self._scales = codes, scales
+            self._codes, self._scales, self._made_on = codes, scales, _stream(self.device)
         quantize_rows(rows, out=(self._codes[first:need, :self.dim], self._scales[first:need]), normalize=normalize)
         self._len = need
         return range(first, need)
@@ -147,6 +175,7 @@ class Int8Rows:
         """Empties the places ``slots`` (whole numbers, any shape).  A slot outside the store changes nothing."""
         if not isinstance(slots, torch.Tensor) or slots.dtype == torch.bool or slots.is_floating_point() or slots.is_complex():
             raise ValueError("slots must be a tensor of whole numbers")
+        self._use()
         at = slots.to(device=self.device, dtype=torch.int64).reshape(-1)
         at = at.masked_fill((at < 0) | (at >= self._len), self._codes.shape[0])
         self._scales.index_fill_(0, at, float("nan"))
@@ -175,6 +204,7 @@ class Int8Rows:
         """search with queries that are quantised already."""
         if not 1 <= int(k) <= _native.CIRCUIT_MAX_K:
             raise ValueError(f"k must be in [1, {_native.CIRCUIT_MAX_K}]")
+        self._use()
         nq, n = query_codes.shape[0], self._len
         none = -(1 << 63)
         best = torch.full((nq, k), none, dtype=torch.int64, device=self.device)

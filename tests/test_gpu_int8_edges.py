@@ -88,3 +88,46 @@ def test_places_stay_on_their_device():
     store = Int8Rows(2, 16, "cuda")
     assert store.device == torch.device("cuda", torch.cuda.current_device()) == store.codes.device
     assert Int8Rows(2, 16).device == store.device
+
+
+def test_growth_keeps_memory_that_another_stream_reads():
+    n, d = 20000, 512
+    store = Int8Rows(0, d, DEV)
+    x = _rows(n, d, 1)
+    store.append(x)
+    want = store.scores(x[:3])
+    old = store._codes.data_ptr(), store._scales.data_ptr()
+    size = store._codes.shape
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        got = store.scores(x[:3])
+    assert store.append(x[:1]) == range(n, n + 1)  # the buffers are full: new ones
+    taken = [torch.full(size, 99, dtype=torch.int8, device=DEV) for _ in range(3)]
+    small = [torch.full((n + 1,), 99.0, device=DEV) for _ in range(3)]
+    assert not side.query()  # the products are still to come
+    assert old[0] not in {t.data_ptr() for t in taken} and old[1] not in {t.data_ptr() for t in small}
+    side.synchronize()
+    assert torch.equal(got, want)
+    assert torch.equal(store.scores(x[:3])[:, :n], want)
+
+
+def test_a_captured_search_outlives_growth():
+    store = Int8Rows(0, 64, DEV)
+    x = _rows(5000, 64, 1)
+    store.append(x)
+    q = x[7:9].clone()
+    want = store.search(q, 3)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = store.search(q, 3)
+        with pytest.raises(RuntimeError):
+            store.append(x)
+    assert store.append(x) == range(5000, 10000)
+    taken = [torch.full((5000, 64), 99, dtype=torch.int8, device=DEV) for _ in range(3)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    del taken

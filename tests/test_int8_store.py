@@ -9,9 +9,16 @@ import torch
 from circuit_rag import CircuitRAG, Int8Rows, _native, int8
 
 
+@pytest.fixture(autouse=True)
+def _one_stream(monkeypatch):
+    monkeypatch.setattr(int8, "_stream", lambda device: 1, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+
 def _host_store(places, dim=8):
     """A store whose buffers lie on the CPU, every place taken (scale 1 + place)."""
     store = Int8Rows.__new__(Int8Rows)
+    store._in_graph, store._captured, store._made_on = False, [], 1
     store.device, store.dim, store._len = torch.device("cpu"), dim, places
     store._codes, store._scales = store._buffers(places)
     store.scales.copy_(torch.arange(places) + 1.0)
@@ -138,3 +145,62 @@ def test_a_growing_store_stays_on_its_device(monkeypatch):
     current[0] = torch.device("cuda", 0)  # another device is current by now
     codes, scales = store._buffers(9)
     assert store.device == torch.device("cuda", 3) and set(asked) == {store.device}
+
+
+def _streams(store, monkeypatch, capturing=False):
+    """Makes `store` believe in streams 1 (its own), 2, ...: returns the current one's number as a list, and the log of
+    (buffer, stream) that the allocator is told of."""
+    now, log = [1], []
+    stream = type("Stream", (), {"__init__": lambda self, n: setattr(self, "n", n)})
+    monkeypatch.setattr(int8, "_stream", lambda device: now[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: stream(now[0]))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, s: log.append((self.data_ptr(), s.n)))
+    monkeypatch.setattr(int8, "quantize_rows", lambda *a, **kw: (torch.zeros(1, 8, dtype=torch.int8), torch.zeros(1)))
+    monkeypatch.setattr(int8, "dequantize_rows", lambda *a, **kw: None)
+    monkeypatch.setattr(int8, "int8_scores", lambda qc, qs, codes, scales, **kw: torch.zeros(len(qc), len(codes)))
+    return now, log
+
+
+CALLS = {
+    "read": lambda s: s.read(torch.zeros(1, dtype=torch.int64)), "scores": lambda s: s.scores(torch.zeros(1, 8)),
+    "search": lambda s: s.search(torch.zeros(1, 8), 2), "search_codes": lambda s: s.search_codes(
+        torch.zeros(1, 8, dtype=torch.int8), torch.zeros(1), 2),
+    "write": lambda s: s.write(torch.zeros(1, 8), torch.zeros(1, dtype=torch.int64)),
+    "remove": lambda s: s.remove(torch.zeros(1, dtype=torch.int64)), "append": lambda s: s.append(torch.zeros(9, 8)),
+    "codes": lambda s: s.codes, "scales": lambda s: s.scales}
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_memory_is_kept_for_the_streams_that_use_it(call, monkeypatch):
+    """Growth drops the old buffers: the allocator knows every stream that may still read or write them."""
+    store = _host_store(4)
+    buffers = {store._codes.data_ptr(), store._scales.data_ptr()}
+    now, log = _streams(store, monkeypatch)
+    CALLS[call](store)
+    assert log == []  # its own stream: the allocator orders that by itself
+    store = _host_store(4)
+    buffers = {store._codes.data_ptr(), store._scales.data_ptr()}
+    now, log = _streams(store, monkeypatch)
+    now[0] = 5
+    CALLS[call](store)
+    assert {b for b, s in log} == buffers and {s for b, s in log} == {5}
+    if call == "append":
+        assert store._made_on == 5 and len(store) == 13
+
+
+def test_buffers_of_a_captured_call_outlive_growth(monkeypatch):
+    store = _host_store(4)
+    now, log = _streams(store, monkeypatch, capturing=True)
+    now[0] = 9
+    CALLS["search"](store)
+    with pytest.raises(RuntimeError):
+        CALLS["append"](store)  # would copy the rows of now at every replay
+    assert len(store) == 4
+    old = store._codes
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    CALLS["append"](store)
+    assert len(store) == 13 and store._captured[0][0] is old
+    CALLS["append"](store)
+    CALLS["append"](store)
+    assert len(store._captured) == 1  # buffers of no graph are not kept
