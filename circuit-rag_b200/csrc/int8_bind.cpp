@@ -13,6 +13,7 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/add.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -87,6 +88,9 @@ void check_dim(int64_t dim) {
 void no_gradient(const Tensor& t, const char* name) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     runtime_error(std::string(name) + " asks for a gradient: the 8-bit rows have no backward pass (use torch.no_grad())");
+  // a dual tensor of forward mode, which torch.no_grad() leaves on
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    runtime_error(std::string(name) + " carries a forward gradient: the 8-bit rows have none (use its primal)");
 }
 
 // A [n, dim] tensor of values that lie next to each other in each row (a copy if they do not).

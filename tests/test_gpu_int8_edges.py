@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from circuit_rag import Int8Rows, dequantize_rows, int8, int8_scores, quantize_rows
+from circuit_rag import Int8Rows, dequantize_rows, int8, int8_scores, quantize_rows, rms_norm_quantize
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +131,25 @@ def test_a_captured_search_outlives_growth():
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     del taken
+
+
+def test_forward_gradients_are_refused():
+    x = _rows(4, 32)
+    codes, scales = quantize_rows(x)
+    with torch.autograd.forward_ad.dual_level():
+        dual = [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, x[0].clone(), scales)]
+        for call in (lambda: quantize_rows(dual[0]), lambda: quantize_rows(dual[0][:, 1:]), lambda: rms_norm_quantize(dual[0]),
+                     lambda: rms_norm_quantize(x, residual=dual[0]), lambda: rms_norm_quantize(x, weight=dual[1]),
+                     lambda: dequantize_rows(codes, dual[2]), lambda: int8_scores(codes, dual[2], codes, scales),
+                     lambda: int8_scores(codes, scales, codes, dual[2]),
+                     lambda: int8_scores(codes, scales, codes, scales, bias=dual[2]),
+                     lambda: quantize_rows(x, out=(codes, dual[2]))):
+            with pytest.raises(RuntimeError):
+                call()
+            with pytest.raises(RuntimeError), torch.no_grad():  # which leaves forward mode on
+                call()
+        plain = torch.autograd.forward_ad.unpack_dual(dual[0]).primal
+        assert torch.equal(quantize_rows(plain)[0], codes)
+    for transform in (lambda f: torch.func.jvp(f, (x,), (x,)), lambda f: torch.func.grad(f)(x), lambda f: torch.func.vmap(f)(x[None])):
+        with pytest.raises(RuntimeError):
+            transform(lambda t: quantize_rows(t)[1].sum())
