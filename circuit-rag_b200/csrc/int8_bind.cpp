@@ -262,6 +262,7 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
       if (out.scalar_type() != type || out.device() != dev || out.dim() != 2 || out.size(0) != n || out.size(1) != dim)
         value_error("out must be of type dtype, of shape [" + std::to_string(n) + ", " + std::to_string(dim) +
                     "], on the rows' device");
+      no_gradient(out, "out");
       check_target(out, "out");
       out_step = step(out);
     } else if (ids.defined()) {
@@ -325,6 +326,7 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t count) {
       if (out.scalar_type() != type || out.device() != dev || out.dim() != 2 || out.size(0) != nq || out.size(1) != n)
         value_error("out must be of type dtype, of shape [" + std::to_string(nq) + ", " + std::to_string(n) +
                     "], on the rows' device");
+      no_gradient(out, "out");
       check_target(out, "out");
       out_step = step(out);
     } else {

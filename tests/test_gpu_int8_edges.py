@@ -153,3 +153,17 @@ def test_forward_gradients_are_refused():
     for transform in (lambda f: torch.func.jvp(f, (x,), (x,)), lambda f: torch.func.grad(f)(x), lambda f: torch.func.vmap(f)(x[None])):
         with pytest.raises(RuntimeError):
             transform(lambda t: quantize_rows(t)[1].sum())
+
+
+def test_results_that_ask_for_a_gradient_are_refused():
+    codes, scales = quantize_rows(_rows(4, 32))
+    values, products = (torch.empty(4, n, device=DEV).requires_grad_() for n in (32, 4))
+    for out in (values, values * 1):  # a leaf, and one with a history that the call would belie
+        with pytest.raises(RuntimeError):
+            dequantize_rows(codes, scales, out=out)
+    for out in (products, products * 1):
+        with pytest.raises(RuntimeError):
+            int8_scores(codes, scales, codes, scales, out=out)
+    with torch.no_grad():
+        assert dequantize_rows(codes, scales, out=values) is values
+        int8_scores(codes, scales, codes, scales, out=products)
