@@ -124,6 +124,11 @@ void check_target(const Tensor& t, const char* name) {
   if (!plain_rows(t)) value_error(std::string(name) + " must be contiguous in each row and its rows must not overlap");
 }
 
+// A given tensor was written: a gradient that kept it for later has to notice.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) {
   return at::detail::empty_cuda(shape, type, dev, std::nullopt);
 }
@@ -219,6 +224,10 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
                  codes.size(0), codes.mutable_data_ptr<int8_t>(), step(codes), scales.mutable_data_ptr<float>(),
                  c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
              "quantize_rows");
+      if (out) {
+        written(codes);
+        written(scales);
+      }
     } else if (n && summed.defined()) {  // a store without rows: nothing is written, the sum is still due
       at::add_out(summed, rows, residual);
     }
@@ -279,6 +288,7 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
                  out.mutable_data_ptr(), type_code(type), out_step,
                  c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
              "dequantize_rows");
+    if (n && have) written(out);
     return have ? given(a[4]) : wrap(out);
   });
 }
@@ -344,6 +354,7 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t count) {
                                     out.mutable_data_ptr(), type_code(type), out_step,
                                     c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
              "int8_scores");
+      if (have) written(out);
     }
     return have ? given(a[6]) : wrap(out);
   });

@@ -167,3 +167,36 @@ def test_results_that_ask_for_a_gradient_are_refused():
     with torch.no_grad():
         assert dequantize_rows(codes, scales, out=values) is values
         int8_scores(codes, scales, codes, scales, out=products)
+
+
+def test_writing_is_known_to_autograd():
+    """What a call writes in place cannot be taken for the values that an earlier operation kept for its gradient."""
+    x = _rows(4, 32)
+    codes, scales = quantize_rows(x)
+    store = Int8Rows(0, 32, DEV)
+    store.append(x)
+    values, products = torch.ones(4, 32, device=DEV), torch.ones(4, 4, device=DEV)
+    slots = torch.arange(4, device=DEV)
+    for kept, write in ((values, lambda: dequantize_rows(codes, scales, out=values)),
+                        (products, lambda: int8_scores(codes, scales, codes, scales, out=products)),
+                        (scales, lambda: quantize_rows(2 * x, out=(codes, scales))),
+                        (scales, lambda: rms_norm_quantize(x, out=(codes, scales))),
+                        (store.scales, lambda: store.write(2 * x, slots))):
+        w = torch.ones_like(kept, requires_grad=True)
+        loss = (w * kept).sum()
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = codes._version, scales._version
+    quantize_rows(x[:0], out=(codes[:0], scales[:0]))
+    int8_scores(codes, scales, codes, scales)
+    dequantize_rows(codes, scales)
+    assert (codes._version, scales._version) == before  # nothing was written
+    quantize_rows(x, out=(codes, scales))
+    assert codes._version > before[0] and scales._version > before[1]
+    with torch.inference_mode():
+        kept = quantize_rows(x)
+        out = torch.empty(4, 32, device=DEV)
+        quantize_rows(2 * x, out=kept)
+    quantize_rows(2 * x, out=kept)  # tensors without a version
+    assert dequantize_rows(*kept, out=out) is out
