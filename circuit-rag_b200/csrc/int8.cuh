@@ -107,6 +107,14 @@ struct Vec {
     memcpy(&word, this, sizeof(W));
     *reinterpret_cast<W*>(row + c) = word;
   }
+  // not zero if an element is not zero
+  __device__ __forceinline__ uint32_t bits() const {
+    uint32_t words[(sizeof(W) + 3) / 4] = {}, all = 0;
+    memcpy(words, this, sizeof(W));
+#pragma unroll
+    for (uint32_t w : words) all |= w;
+    return all;
+  }
 };
 
 // ---------------------------------------------------------------- host side

@@ -62,8 +62,8 @@ __device__ __forceinline__ RowSums reduce(RowSums r) {
 // nearest integer.  u, top and the division are off by 2^-24 of their size each and
 // hi and lo by another, so the real quotient lies between u * lo and u * hi: where
 // both give the same integer it is the code, where not (within 127 2^-21 = 6e-5 of
-// a half: 0.006 % of the values) 254 v w is compared with (2 n + 1) top in 64 bits,
-// in which v * w is exact.
+// a half: 0.006 % of the values) 254 v w is compared with (2 n + 1) top exactly
+// (exact_codes).
 //
 // 16-bit values without a weight have m < 2^11 steps of their exponent, as has top
 // (ma): 127 v / top = 127 mv / (ma 2^k) is either a half, or 1 / (2 ma 2^k) >=
@@ -139,26 +139,82 @@ __device__ __noinline__ float wide_range_scale(const T* src, int d, float top, f
   return (float)((double)top / 127.0 / sqrt(ldexp((double)m.ss * (double)inv_n, 2 * e) + (double)eps));
 }
 
-// Rare: codes of elements [c, c + e), halves decided in 64 bits (a: the row's exact
-// maximum; hi = 0: the row is too small for 32 bits throughout).
+template <typename T>
+__device__ __forceinline__ float weight(const QuantizeParams& P, int i) {
+  if (!P.w) return 1.f;
+  return P.w_f32 ? reinterpret_cast<const float*>(P.w)[i] : RowType<T>::get(reinterpret_cast<const T*>(P.w)[i]);
+}
+// n or n + 1, as 254 u lies below or above (2 n + 1) a, of a half the even one.  Both
+// products take up to 56 bits: each is held as its rounded value and the rest, which an
+// FMA gives.
+__device__ __forceinline__ int nearest(double u, double a, int n) {
+  const double m = (double)(2 * n + 1), l = __dmul_rn(254.0, u), r = __dmul_rn(m, a);
+  const double above = __dadd_rn(__dsub_rn(l, r), __dsub_rn(__fma_rn(254.0, u, -l), __fma_rn(m, a, -r)));
+  return n + (above > 0.0 || (above == 0.0 && (n & 1)));
+}
+
+// Rare: codes of elements [c, c + e) from the row's exact maximum a, halves decided
+// exactly (hi = 0: the row is too small for 32 bits throughout, and n is the quotient
+// rounded down, or one off next to a whole number).
 template <typename T>
 __device__ __noinline__ void exact_codes(const QuantizeParams& P, const T* src, int8_t* out, int c, int e, double a,
                                          float hi, float lo) {
   for (int i = c; i < c + e; ++i) {
-    float w = 1.f;
-    if (P.w) w = P.w_f32 ? reinterpret_cast<const float*>(P.w)[i] : RowType<T>::get(reinterpret_cast<const T*>(P.w)[i]);
-    const float v = RowType<T>::get(src[i]), t = v * w;
-    const double u = fabs((double)v * (double)w);
-    int n;
-    if (hi == 0.f) {
-      n = (int)rint(u * 127.0 / a);
-    } else {
-      const int n0 = (int)(fmaf(fabsf(t), lo, ROUNDER) - ROUNDER), n1 = (int)(fmaf(fabsf(t), hi, ROUNDER) - ROUNDER);
-      const double above = 254.0 * u - (double)(2 * n0 + 1) * a;
-      n = n0 == n1 ? n0 : above > 0.0 ? n1 : above < 0.0 ? n0 : n0 + (n0 & 1);
+    const float v = RowType<T>::get(src[i]), w = weight<T>(P, i), t = fabsf(v * w);
+    int n = (int)(fmaf(t, lo, ROUNDER) - ROUNDER);
+    if (hi == 0.f || n != (int)(fmaf(t, hi, ROUNDER) - ROUNDER)) {
+      const double u = fabs((double)v * (double)w);  // 48 bits
+      n = nearest(u, a, hi == 0.f ? (int)(u * 127.0 / a) : n);
     }
-    out[i] = (int8_t)(t < 0.f ? -n : n);
+    out[i] = (int8_t)(v * w < 0.f ? -n : n);
   }
+}
+
+// Rare: a row whose largest product with the weights is so small that 32 bits hold it
+// with few digits or not at all: its codes and scale in 64 bits, over what the kernel
+// wrote for it (each thread its own elements).  All threads of a warp or block come
+// here; rows that are not faint, or have no place (dst < 0), are left alone.
+template <typename T, int E, int G>
+__device__ __noinline__ void faint_row(const QuantizeParams& P, const T* src, int d, bool faint, int64_t dst) {
+  const int lane = threadIdx.x % G;
+  uint32_t bits = 0;  // rows of zeros end here
+  for (int c = lane * E; c < d && faint; c += G * E) bits |= Vec<T, E>::load(src, c, d).bits();
+  if constexpr (G > 32) bits = __syncthreads_or(bits);
+  else bits = __any_sync(FULL_MASK, bits);
+  if (!bits) return;
+  RowSums m{0.f, 0.f, 0.f};
+  double a = 0.0;
+  for (int c = lane * E; c < d; c += G * E)
+    for (int i = 0; i < E; ++i) {
+      m.top = max_abs_nan(m.top, RowType<T>::get(src[c + i]));
+      a = fmax(a, fabs((double)RowType<T>::get(src[c + i]) * (double)weight<T>(P, c + i)));
+    }
+  m = reduce<G, false, false>(m);
+#pragma unroll
+  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) a = fmax(a, __shfl_xor_sync(FULL_MASK, a, o));
+  if constexpr (G > 32) {
+    __shared__ double part[G / 32];
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+    __syncthreads();
+    for (int w = 0; w < G / 32; ++w) a = fmax(a, part[w]);
+  }
+  const int e = faint && m.top > 0.f ? ilogbf(m.top) : 0;
+  for (int c = lane * E; c < d; c += G * E)
+    for (int i = 0; i < E; ++i) {
+      const float q = ldexpf(RowType<T>::get(src[c + i]), -e);
+      m.ss = fmaf(q, q, m.ss);
+    }
+  m = reduce<G, false, true>(m);
+  if (!faint || dst < 0 || a == 0.0) return;  // a = 0: the zeros that the kernel wrote
+  if (lane == 0)
+    P.scales[dst] = (float)(a / 127.0 / sqrt(ldexp((double)m.ss * (double)P.inv_n, 2 * e) + (double)P.eps));
+  int8_t* out = P.codes + dst * P.code_stride;
+  for (int c = lane * E; c < d; c += G * E)
+    for (int i = c; i < c + E; ++i) {
+      const double p = (double)RowType<T>::get(src[i]) * (double)weight<T>(P, i), u = fabs(p);
+      const int n = nearest(u, a, (int)(u * 127.0 / a));
+      out[i] = (int8_t)(p < 0.0 ? -n : n);
+    }
 }
 
 // G threads a row (8 or 16 lanes, a warp, or a block), the row in NV vectors of E
@@ -268,9 +324,12 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
       if (odd) scale = s;
     }
   }
-  if (dst < 0) return;  // nothing below needs the other lanes
+  // products below 2^-100 lose their last digits (the FMA's rest no longer fits 32 bits)
+  const bool faint = FULL && P.w && r.top < 1e-30f;
+  const bool again = FULL && (G >= 32 ? faint : (bool)__any_sync(FULL_MASK, faint));
+  if (dst < 0 && (G >= 32 || !again)) return;  // nothing below needs the other lanes, but for the last step
   if (bad) scale = __uint_as_float(0x7fffffffu);  // a NaN without the sign that marks claims
-  if (lane == 0) P.scales[dst] = scale;
+  if (lane == 0 && dst >= 0) P.scales[dst] = scale;
 
   int8_t* out = P.codes + dst * P.code_stride;
   // rows so small that 127 / top may overflow take the 64-bit quotient throughout
@@ -284,7 +343,7 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * G + lane) * E;
-    if (c >= d) break;
+    if (c >= d || (FULL && dst < 0)) break;
     [[maybe_unused]] float w[FULL ? E : 1];
     uint32_t n[E];
     if (alone) {
@@ -305,13 +364,16 @@ __global__ void __launch_bounds__(row_threads(G)) k_quantize_rows(const __grid_c
     }
     store_codes<E>(out, c, n, bad);
   }
-  if (unsure && !bad) {
+  if (unsure && !bad && !faint && dst >= 0) {
     const double a = (double)r.top + (double)r.low;
     for (int k = 0; k < NV; ++k)
       if (unsure >> k & 1u) {
         const int c = (k * G + lane) * E;
         if (c < d) exact_codes<T>(P, x, out, c, E, a, hi, lo);
       }
+  }
+  if constexpr (FULL) {
+    if (again) faint_row<T, E, G>(P, x, d, faint, dst);
   }
 }
 
