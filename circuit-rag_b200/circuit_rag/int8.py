@@ -204,6 +204,9 @@ class Int8Rows:
         """search with queries that are quantised already."""
         if not 1 <= int(k) <= _native.CIRCUIT_MAX_K:
             raise ValueError(f"k must be in [1, {_native.CIRCUIT_MAX_K}]")
+        if (query_codes.ndim != 2 or query_codes.dtype != torch.int8 or query_codes.shape[1] != self.dim or
+                query_scales.dtype != torch.float32 or query_scales.shape != query_codes.shape[:1]):
+            raise ValueError("queries must be int8 codes [nq, dim] and float32 scales [nq]")
         self._use()
         nq, n = query_codes.shape[0], self._len
         none = -(1 << 63)

@@ -204,3 +204,17 @@ def test_buffers_of_a_captured_call_outlive_growth(monkeypatch):
     CALLS["append"](store)
     CALLS["append"](store)
     assert len(store._captured) == 1  # buffers of no graph are not kept
+
+
+@pytest.mark.parametrize("places", [0, 4])
+def test_search_checks_its_queries(places):
+    """Also where nothing is multiplied: a store without places, no queries."""
+    store = _host_store(places)
+    good = torch.zeros(2, 8, dtype=torch.int8), torch.zeros(2)
+    for codes, scales in ((torch.zeros(2, 9, dtype=torch.int8), good[1]), (good[0], torch.zeros(3)), (good[0][0], good[1]),
+                          (good[0].float(), good[1]), (good[0], good[1].double()), (good[0], good[1][:, None]),
+                          (torch.zeros(0, 9, dtype=torch.int8), torch.zeros(0))):
+        with pytest.raises(ValueError):
+            store.search_codes(codes, scales, k=2)
+    scores, ids = store.search_codes(good[0][:0], good[1][:0], k=2)
+    assert scores.shape == ids.shape == (0, 2) and ids.dtype == torch.int32
