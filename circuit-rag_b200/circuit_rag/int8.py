@@ -197,8 +197,8 @@ class Int8Rows:
         gave up a wait, see check_products, or left the range of float32) comes first, with score NaN."""
         return self.search_codes(*quantize_rows(queries, normalize=normalize), k=k)
 
-    # scores of a block of rows that are ranked at a time
-    _BLOCK = 1 << 25
+    # scores that are ranked at a time: of so many rows at least, so of so many queries at most
+    _BLOCK, _BLOCK_ROWS = 1 << 25, 1 << 14
 
     def search_codes(self, query_codes: torch.Tensor, query_scales: torch.Tensor, k: int = 10):
         """search with queries that are quantised already."""
@@ -209,9 +209,13 @@ class Int8Rows:
             raise ValueError("queries must be int8 codes [nq, dim] and float32 scales [nq]")
         self._use()
         nq, n = query_codes.shape[0], self._len
+        most = max(1, self._BLOCK // self._BLOCK_ROWS)
+        if nq > most:
+            parts = [self.search_codes(query_codes[a:a + most], query_scales[a:a + most], k) for a in range(0, nq, most)]
+            return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
         none = -(1 << 63)
         best = torch.full((nq, k), none, dtype=torch.int64, device=self.device)
-        block = max(1 << 14, self._BLOCK // max(1, nq))
+        block = max(self._BLOCK_ROWS, self._BLOCK // max(1, nq))
         for a in range(0, n if nq else 0, block):
             b = min(n, a + block)
             s = int8_scores(query_codes, query_scales, self._codes[a:b, :self.dim], self._scales[a:b])

@@ -200,3 +200,20 @@ def test_writing_is_known_to_autograd():
         quantize_rows(2 * x, out=kept)
     quantize_rows(2 * x, out=kept)  # tensors without a version
     assert dequantize_rows(*kept, out=out) is out
+
+
+def test_search_of_many_queries_in_bounded_memory():
+    store = Int8Rows(0, 32, DEV)
+    store.append(_rows(20000, 32, 1))
+    q = _rows(70001, 32, 2)  # more than a call of the products takes
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    scores, ids = store.search(q, 5)
+    torch.cuda.synchronize()
+    # 2^25 scores of 4 bytes, a few whole numbers of 8 of each, and a sort of these
+    assert torch.cuda.max_memory_allocated() - before < 16 * 8 * (1 << 25)
+    assert scores.shape == ids.shape == (70001, 5)
+    for a in (0, 2040, 2048, 65535, 69990):
+        want = store.search(q[a:a + 11], 5)
+        assert torch.equal(ids[a:a + 11], want[1]) and torch.equal(scores[a:a + 11], want[0])

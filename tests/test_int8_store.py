@@ -218,3 +218,17 @@ def test_search_checks_its_queries(places):
             store.search_codes(codes, scales, k=2)
     scores, ids = store.search_codes(good[0][:0], good[1][:0], k=2)
     assert scores.shape == ids.shape == (0, 2) and ids.dtype == torch.int32
+
+
+def test_search_of_many_queries_keeps_its_block(monkeypatch):
+    """The scores ranked at a time stay within a block however many queries there are."""
+    store, most = _host_store(5000), []
+    monkeypatch.setattr(int8, "int8_scores", lambda qc, qs, codes, scales: most.append(len(qc) * len(codes)) or
+                        qs[:, None] * scales[None])
+    store._BLOCK = 1 << 16
+    for nq in (1, 3, 700, 65535 // 16):
+        scales = 1.0 + torch.arange(nq) % 7
+        scores, ids = store.search_codes(torch.zeros(nq, 8, dtype=torch.int8), scales, k=3)
+        assert max(most) <= 1 << 16, nq
+        assert ids.tolist() == [[4999, 4998, 4997]] * nq
+        assert torch.equal(scores, scales[:, None] * torch.tensor([5000.0, 4999.0, 4998.0]))
