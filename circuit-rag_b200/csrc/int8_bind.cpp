@@ -61,10 +61,21 @@ void native(int rc, const char* what) {
   throw Refused{type ? type : PyExc_RuntimeError, std::move(m)};  // the class lives as long as its module
 }
 
-Tensor cuda_tensor(PyObject* o, const char* name) {
+Tensor given_tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) runtime_error(std::string(name) + " must be CUDA tensor");
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda()) runtime_error(std::string(name) + " must be CUDA tensor");
+  return t;
+}
+// A tensor to read: a view that stands for the negative of its memory (the imaginary part of a conjugate) as a copy.
+Tensor cuda_tensor(PyObject* o, const char* name) {
+  Tensor t = given_tensor(o, name);
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+// A tensor to write.
+Tensor cuda_target(PyObject* o, const char* name) {
+  Tensor t = given_tensor(o, name);
+  if (t.is_neg()) value_error(std::string(name) + " must not be a view of its negative");
   return t;
 }
 
@@ -200,8 +211,8 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
     if (out) {
       if (!PyTuple_Check(a[6]) || PyTuple_GET_SIZE(a[6]) != 2) value_error("out must be a tuple (codes, scales)");
-      codes = cuda_tensor(PyTuple_GET_ITEM(a[6], 0), "out codes");
-      scales = cuda_tensor(PyTuple_GET_ITEM(a[6], 1), "out scales");
+      codes = cuda_target(PyTuple_GET_ITEM(a[6], 0), "out codes");
+      scales = cuda_target(PyTuple_GET_ITEM(a[6], 1), "out scales");
       check_pair(codes, scales, "out");
       check_target(codes, "out codes");
       if (!scales.is_contiguous()) value_error("out scales must be contiguous");
@@ -267,7 +278,7 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
     const bool have = a[4] != Py_None;
     if (have) {
-      out = cuda_tensor(a[4], "out");
+      out = cuda_target(a[4], "out");
       if (out.scalar_type() != type || out.device() != dev || out.dim() != 2 || out.size(0) != n || out.size(1) != dim)
         value_error("out must be of type dtype, of shape [" + std::to_string(n) + ", " + std::to_string(dim) +
                     "], on the rows' device");
@@ -332,7 +343,7 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t count) {
     int64_t out_step = n;
     const bool have = a[6] != Py_None;
     if (have) {
-      out = cuda_tensor(a[6], "out");
+      out = cuda_target(a[6], "out");
       if (out.scalar_type() != type || out.device() != dev || out.dim() != 2 || out.size(0) != nq || out.size(1) != n)
         value_error("out must be of type dtype, of shape [" + std::to_string(nq) + ", " + std::to_string(n) +
                     "], on the rows' device");

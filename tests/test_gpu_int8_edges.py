@@ -217,3 +217,31 @@ def test_search_of_many_queries_in_bounded_memory():
     for a in (0, 2040, 2048, 65535, 69990):
         want = store.search(q[a:a + 11], 5)
         assert torch.equal(ids[a:a + 11], want[1]) and torch.equal(scores[a:a + 11], want[0])
+
+
+def test_tensors_that_stand_for_their_negative():
+    """The imaginary part of a conjugate lies in memory with the other sign."""
+    z = torch.complex(_rows(300, 40, 1), _rows(300, 40, 2))
+    for cut in (slice(0, 40), slice(0, 1)):  # one value a row: any stride is read in place
+        rows = z[:, cut].conj().imag
+        assert rows.is_neg()
+        want = quantize_rows(rows.resolve_neg().contiguous())
+        for got in (quantize_rows(rows), quantize_rows(torch._neg_view(-rows.clone()))):
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        weight = torch.complex(rows[0].clone(), rows[1].clone()).conj().imag
+        got = rms_norm_quantize(rows, residual=rows, weight=weight)
+        plain = rows.clone()
+        for a, b in zip(got, rms_norm_quantize(plain, residual=plain, weight=weight.clone())):
+            assert torch.equal(a, b)
+    codes, scales = want
+    bias = z[:, 0].conj().imag
+    assert torch.equal(int8_scores(codes, scales, codes, scales, bias=bias),
+                       int8_scores(codes, scales, codes, scales, bias=bias.clone()))
+    assert torch.equal(int8_scores(codes, scales, codes, scales, bias=torch._neg_view(-bias)),
+                       int8_scores(codes, scales, codes, scales, bias=bias.clone()))
+    for call in (lambda out: dequantize_rows(codes, scales, out=out),
+                 lambda out: int8_scores(codes, scales, codes[:1], scales[:1], out=out)):
+        with pytest.raises(ValueError):
+            call(z[:, :1].conj().imag)
+    with pytest.raises(ValueError):
+        quantize_rows(plain, out=(codes, torch._neg_view(scales)))
