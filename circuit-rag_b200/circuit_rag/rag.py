@@ -100,7 +100,7 @@ class CircuitRAG:
         relevant; the query (at unit length) is moved by their mean before it is compared."""
         if feedback and self.rows != "int8":
             raise ValueError('feedback needs rows="int8"')
-        if self.index is None and self.store is None:
+        if (self.index is None and self.store is None) or not self.texts:
             return []
         q = torch.from_numpy(np.asarray(self._embed([query]), dtype=np.float32)[0])
         k = min(k, len(self.texts))

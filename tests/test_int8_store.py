@@ -232,3 +232,9 @@ def test_search_of_many_queries_keeps_its_block(monkeypatch):
         assert max(most) <= 1 << 16, nq
         assert ids.tolist() == [[4999, 4998, 4997]] * nq
         assert torch.equal(scores, scales[:, None] * torch.tensor([5000.0, 4999.0, 4998.0]))
+
+
+def test_rag_without_documents_finds_nothing():
+    rag = CircuitRAG(device="cpu", embed_fn=lambda texts: np.ones((len(texts), 8), np.float32), rows="int8")
+    rag.store = _host_store(0)  # as adding an empty list leaves it
+    assert rag.search("q") == []
