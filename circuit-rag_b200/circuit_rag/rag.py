@@ -121,7 +121,8 @@ class CircuitRAG:
         if feedback:
             ids = torch.tensor(feedback, dtype=torch.int64, device=q.device)
             mean = self.store.read(ids).mean(0, keepdim=True)
-            q = q / q.norm().clamp(min=torch.finfo(q.dtype).tiny)  # as long as each document
+            wide = q.double()  # squares of 32 bits may leave their range
+            q = (wide / wide.norm().clamp(min=torch.finfo(wide.dtype).tiny)).to(q.dtype)  # as long as each document
             # the root-mean-square norm times dim^-1/2: unit length again
             unit = torch.full((self.store.dim,), self.store.dim ** -0.5, device=q.device)
             codes, scales, _ = rms_norm_quantize(q, residual=mean, weight=unit, eps=0.0)

@@ -1,8 +1,9 @@
 """8-bit rows on the GPU: the calls at the edge of what the documents allow."""
+import numpy as np
 import pytest
 import torch
 
-from circuit_rag import Int8Rows, dequantize_rows, int8, int8_scores, quantize_rows, rms_norm_quantize
+from circuit_rag import CircuitRAG, Int8Rows, dequantize_rows, int8, int8_scores, quantize_rows, rms_norm_quantize
 
 pytestmark = pytest.mark.gpu
 
@@ -245,3 +246,23 @@ def test_tensors_that_stand_for_their_negative():
             call(z[:, :1].conj().imag)
     with pytest.raises(ValueError):
         quantize_rows(plain, out=(codes, torch._neg_view(scales)))
+
+
+def test_feedback_does_not_depend_on_the_length_of_the_query():
+    g = torch.Generator().manual_seed(3)
+    vectors = {f"doc {i}": torch.randn(48, generator=g).numpy() for i in range(300)}
+    sizes = {"": 1.0, " long": 1e30, " short": 1e-30}
+
+    def embed(texts):
+        found = [(vectors[t[:t.index("#")]], sizes[t[t.index("#") + 1:]]) for t in texts]
+        return np.stack([v * np.float32(size) for v, size in found])
+
+    rag = CircuitRAG(device=DEV, embed_fn=embed, rows="int8")
+    rag.add_documents([f"doc {i}#" for i in range(300)])
+    want = rag.search("doc 5#", k=4, feedback=[42, 7])
+    assert want[0].id == 5  # random directions: 1 / 1.5^(1/2) against its own document
+    for size in (" long", " short"):
+        got = rag.search("doc 5#" + size, k=4, feedback=[42, 7])
+        assert [r.id for r in got] == [r.id for r in want]
+        # the same query but for the rounding of its values: a code may differ by one, the score by less than 1 / 127 for it
+        assert all(abs(a.score - b.score) < 0.02 for a, b in zip(got, want))
