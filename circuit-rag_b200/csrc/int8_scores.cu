@@ -660,10 +660,15 @@ int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const fl
 }
 
 int circuit_op_int8_status(void* stream) {
-  int rc = check(cudaStreamSynchronize((cudaStream_t)stream), "int8_status"), bits = 0;
+  cudaStream_t st = (cudaStream_t)stream;  // copies on it too: others would wait for the work of every stream
+  int bits = 0;
   const int none = 0;
-  if (!rc) rc = check(cudaMemcpyFromSymbol(&bits, g_error, sizeof(int)), "int8_status");
-  if (!rc && bits) rc = check(cudaMemcpyToSymbol(g_error, &none, sizeof(int)), "int8_status");
+  int rc = check(cudaMemcpyFromSymbolAsync(&bits, g_error, sizeof(int), 0, cudaMemcpyDeviceToHost, st), "int8_status");
+  if (!rc) rc = check(cudaStreamSynchronize(st), "int8_status");
+  if (!rc && bits) {
+    rc = check(cudaMemcpyToSymbolAsync(g_error, &none, sizeof(int), 0, cudaMemcpyHostToDevice, st), "int8_status");
+    if (!rc) rc = check(cudaStreamSynchronize(st), "int8_status");
+  }
   if (rc || !bits) return rc;
   bad("int8_scores: a bounded wait on the device gave up; its results are NaN");
   return CIRCUIT_ERR_TIMEOUT;

@@ -266,3 +266,14 @@ def test_feedback_does_not_depend_on_the_length_of_the_query():
         assert [r.id for r in got] == [r.id for r in want]
         # the same query but for the rounding of its values: a code may differ by one, the score by less than 1 / 127 for it
         assert all(abs(a.score - b.score) < 0.02 for a, b in zip(got, want))
+
+
+def test_status_waits_for_its_stream_only():
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)  # about a fifth of a second on the default stream
+    with torch.cuda.stream(side):
+        int8.check_products()
+    assert not torch.cuda.default_stream().query()
+    int8.check_products()
+    assert torch.cuda.default_stream().query()
