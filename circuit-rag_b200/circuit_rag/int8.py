@@ -219,11 +219,12 @@ class Int8Rows:
         for a in range(0, n if nq else 0, block):
             b = min(n, a + block)
             s = int8_scores(query_codes, query_scales, self._codes[a:b, :self.dim], self._scales[a:b])
-            # one whole number a score: the order of floats (NaN above all, as the kernel writes it) in the upper half,
-            # the lower place first in the lower half
-            bits = s.view(torch.int32).to(torch.int64)
-            bits ^= (bits >> 31) & 0x7FFFFFFF
-            key = (bits << 32) + (0xFFFFFFFF - torch.arange(a, b, device=self.device))
+            # one whole number a score: the order of floats (both zeros as 0, NaN above all, as the kernel writes it) in
+            # the upper half, the lower place first in the lower half
+            order = s.add_(0.0).view(torch.int32)
+            order ^= (order >> 31) & 0x7FFFFFFF
+            last = 0xFFFFFFFF
+            key = torch.add(torch.arange(last - a, last - b, -1, device=self.device), order, alpha=1 << 32)
             key.masked_fill_(self._scales[a:b].isnan(), none)
             best = torch.cat([best, key], 1).topk(k, dim=1).values
         empty = (best == none) | query_scales.isnan()[:, None]

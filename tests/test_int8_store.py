@@ -238,3 +238,13 @@ def test_rag_without_documents_finds_nothing():
     rag = CircuitRAG(device="cpu", embed_fn=lambda texts: np.ones((len(texts), 8), np.float32), rows="int8")
     rag.store = _host_store(0)  # as adding an empty list leaves it
     assert rag.search("q") == []
+
+
+def test_zeros_of_both_signs_are_a_tie(monkeypatch):
+    """A product that underflows keeps its sign; it is no smaller than a zero."""
+    store = _host_store(6)
+    tiny = 2.0 ** -149
+    products = torch.tensor([[-0.0, 0.0, -0.0, tiny, -tiny, 0.0], [-tiny, -0.0, -2.0, -1.0, -math.inf, math.inf]])
+    scores, ids = _search(store, products, torch.ones(2), 6, monkeypatch)
+    assert ids.tolist() == [[3, 0, 1, 2, 5, 4], [5, 1, 0, 3, 2, 4]]
+    assert scores.tolist() == [[tiny, 0.0, 0.0, 0.0, 0.0, -tiny], [math.inf, 0.0, -tiny, -1.0, -2.0, -math.inf]]
