@@ -122,32 +122,32 @@ class Int8Rows:
         # one scale more than places: what is meant for no place goes there
         return codes, torch.full((n + 1,), float("nan"), dtype=torch.float32, device=self.device)
 
-    def _use(self) -> None:
-        """The current stream uses the buffers: their memory is kept for it when a growing store drops them."""
-        if _stream(self.device) != self._made_on:
+    def _use(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Codes and scales for the current stream: their memory is kept for it when a growing store drops them."""
+        now = _stream(self.device)
+        if now != self._made_on:
             stream = torch.cuda.current_stream(self.device)
             self._codes.record_stream(stream)
             self._scales.record_stream(stream)
-        if torch.cuda.is_current_stream_capturing():
+        if now and torch.cuda.is_current_stream_capturing():  # never the default stream, 0
             self._in_graph = True
+        return self._codes[:self._len, :self.dim], self._scales[:self._len]
 
     def __len__(self) -> int:
         return self._len
 
     @property
     def codes(self) -> torch.Tensor:
-        self._use()
-        return self._codes[:self._len, :self.dim]
+        return self._use()[0]
 
     @property
     def scales(self) -> torch.Tensor:
-        self._use()
-        return self._scales[:self._len]
+        return self._use()[1]
 
     def write(self, rows: torch.Tensor, slots: torch.Tensor, normalize: bool = False) -> None:
         """Quantises rows [n, dim] into places slots [n] (int32 or int64).  A slot outside the store writes nothing, of
         equal slots the last row stays."""
-        quantize_rows(rows, slots=slots, out=(self.codes, self.scales), normalize=normalize)
+        quantize_rows(rows, slots=slots, out=self._use(), normalize=normalize)
 
     def append(self, rows: torch.Tensor, normalize: bool = False) -> range:
         """Adds rows [n, dim] in new places at the end and returns these places."""
@@ -182,13 +182,13 @@ class Int8Rows:
 
     def read(self, ids: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The rows at ``ids`` (any shape, as a search returns them; -1 gives zeros)."""
-        return dequantize_rows(self.codes, self.scales, ids, dtype=dtype)
+        return dequantize_rows(*self._use(), ids, dtype=dtype)
 
     def scores(self, queries: torch.Tensor, bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float32,
                normalize: bool = False) -> torch.Tensor:
         """Products [nq, len] of queries [nq, dim], quantised row by row, with all places."""
         codes, scales = quantize_rows(queries, normalize=normalize)
-        return int8_scores(codes, scales, self.codes, self.scales, bias=bias, dtype=dtype)
+        return int8_scores(codes, scales, *self._use(), bias=bias, dtype=dtype)
 
     def search(self, queries: torch.Tensor, k: int = 10, normalize: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
         """The k best places of each query [nq, dim] by its product with the stored rows: (scores [nq, k] descending,
@@ -207,29 +207,35 @@ class Int8Rows:
         if (query_codes.ndim != 2 or query_codes.dtype != torch.int8 or query_codes.shape[1] != self.dim or
                 query_scales.dtype != torch.float32 or query_scales.shape != query_codes.shape[:1]):
             raise ValueError("queries must be int8 codes [nq, dim] and float32 scales [nq]")
-        self._use()
+        codes, scales = self._use()
         nq, n = query_codes.shape[0], self._len
         most = max(1, self._BLOCK // self._BLOCK_ROWS)
         if nq > most:
             parts = [self.search_codes(query_codes[a:a + most], query_scales[a:a + most], k) for a in range(0, nq, most)]
             return torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts])
         none = -(1 << 63)
-        best = torch.full((nq, k), none, dtype=torch.int64, device=self.device)
+        best = None
         block = max(self._BLOCK_ROWS, self._BLOCK // max(1, nq))
         for a in range(0, n if nq else 0, block):
             b = min(n, a + block)
-            s = int8_scores(query_codes, query_scales, self._codes[a:b, :self.dim], self._scales[a:b])
+            s = int8_scores(query_codes, query_scales, codes[a:b], scales[a:b])
             # one whole number a score: the order of floats (both zeros as 0, NaN above all, as the kernel writes it) in
             # the upper half, the lower place first in the lower half
             order = s.add_(0.0).view(torch.int32)
             order ^= (order >> 31) & 0x7FFFFFFF
             last = 0xFFFFFFFF
             key = torch.add(torch.arange(last - a, last - b, -1, device=self.device), order, alpha=1 << 32)
-            key.masked_fill_(self._scales[a:b].isnan(), none)
-            best = torch.cat([best, key], 1).topk(k, dim=1).values
+            key.masked_fill_(scales[a:b].isnan(), none)
+            if best is not None:
+                key = torch.cat([best, key], 1)
+            best = key.topk(min(k, key.shape[1]), dim=1).values
+        if best is None or best.shape[1] < k:  # fewer places than results
+            more = k - (0 if best is None else best.shape[1])
+            blank = torch.full((nq, more), none, dtype=torch.int64, device=self.device)
+            best = blank if best is None else torch.cat([best, blank], 1)
         empty = (best == none) | query_scales.isnan()[:, None]
         bits = best >> 32
         bits ^= (bits >> 31) & 0x7FFFFFFF
         scores = bits.to(torch.int32).view(torch.float32).masked_fill_(empty, float("-inf"))
-        ids = (0xFFFFFFFF - (best & 0xFFFFFFFF)).to(torch.int32).masked_fill_(empty, -1)
+        ids = (~best).to(torch.int32).masked_fill_(empty, -1)  # the lower half
         return scores, ids
