@@ -98,7 +98,8 @@ class Int8Rows:
 
     ``codes`` [len, dim] and ``scales`` [len] are what int8_scores and dequantize_rows take; a place without a row has
     scale NaN, reads as NaN and is never a search result.  Calls on one store are ordered by their streams: writing
-    places while another stream reads them is the caller's to order.  An append that outgrows the buffers moves every
+    places while another stream reads them is the caller's to order.  One thread at a time writes, appends or removes;
+    others may read and search meanwhile.  An append that outgrows the buffers moves every
     place to new ones, so to later calls on other streams it counts as writing every place; calls that are under way
     elsewhere still have the old buffers, which are not used again before these calls are done.  ``codes`` and
     ``scales`` taken before an append, and calls captured into a graph before it, see the places as they were then:
@@ -113,9 +114,9 @@ class Int8Rows:
         self.dim = int(dim)
         self._len = int(places)
         self._in_graph, self._captured = False, []  # a captured call uses the buffers; older buffers of such calls
-        self._codes, self._scales = self._buffers(self._len)
-        self.device = self._codes.device  # with its index: the current device may change
-        self._made_on = _stream(self.device)
+        codes, scales = self._buffers(self._len)
+        self.device = codes.device  # with its index: the current device may change
+        self._made = codes, scales, _stream(self.device)  # replaced as a whole: threads that search see one or the other
 
     def _buffers(self, n: int):
         codes = torch.zeros((n, (self.dim + 15) // 16 * 16), dtype=torch.int8, device=self.device)
@@ -124,14 +125,15 @@ class Int8Rows:
 
     def _use(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """Codes and scales for the current stream: their memory is kept for it when a growing store drops them."""
-        now = _stream(self.device)
-        if now != self._made_on:
+        n, now = self._len, _stream(self.device)  # the length first: later buffers hold as many places
+        codes, scales, made_on = self._made
+        if now != made_on:
             stream = torch.cuda.current_stream(self.device)
-            self._codes.record_stream(stream)
-            self._scales.record_stream(stream)
+            codes.record_stream(stream)
+            scales.record_stream(stream)
         if now and torch.cuda.is_current_stream_capturing():  # never the default stream, 0
             self._in_graph = True
-        return self._codes[:self._len, :self.dim], self._scales[:self._len]
+        return codes[:n, :self.dim], scales[:n]
 
     def __len__(self) -> int:
         return self._len
@@ -157,17 +159,18 @@ class Int8Rows:
         if need >= 2 ** 31:
             raise ValueError("a store holds less than 2^31 rows")
         self._use()
-        if need > self._codes.shape[0]:
+        codes, scales, _ = self._made
+        if need > codes.shape[0]:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a store does not grow inside a graph: each replay would copy the old rows")
             if self._in_graph:
-                self._captured.append((self._codes, self._scales))
+                self._captured.append((codes, scales))
                 self._in_graph = False
-            codes, scales = self._buffers(max(need, 2 * self._codes.shape[0]))
-            codes[:first].copy_(self._codes[:first])
-            scales[:first].copy_(self._scales[:first])
-            self._codes, self._scales, self._made_on = codes, scales, _stream(self.device)
-        quantize_rows(rows, out=(self._codes[first:need, :self.dim], self._scales[first:need]), normalize=normalize)
+            old, (codes, scales) = (codes, scales), self._buffers(max(need, 2 * codes.shape[0]))
+            codes[:first].copy_(old[0][:first])
+            scales[:first].copy_(old[1][:first])
+            self._made = codes, scales, _stream(self.device)
+        quantize_rows(rows, out=(codes[first:need, :self.dim], scales[first:need]), normalize=normalize)
         self._len = need
         return range(first, need)
 
@@ -176,9 +179,10 @@ class Int8Rows:
         if not isinstance(slots, torch.Tensor) or slots.dtype == torch.bool or slots.is_floating_point() or slots.is_complex():
             raise ValueError("slots must be a tensor of whole numbers")
         self._use()
+        codes, scales, _ = self._made
         at = slots.to(device=self.device, dtype=torch.int64).reshape(-1)
-        at = at.masked_fill((at < 0) | (at >= self._len), self._codes.shape[0])
-        self._scales.index_fill_(0, at, float("nan"))
+        at = at.masked_fill((at < 0) | (at >= self._len), codes.shape[0])
+        scales.index_fill_(0, at, float("nan"))
 
     def read(self, ids: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The rows at ``ids`` (any shape, as a search returns them; -1 gives zeros)."""
@@ -208,7 +212,7 @@ class Int8Rows:
                 query_scales.dtype != torch.float32 or query_scales.shape != query_codes.shape[:1]):
             raise ValueError("queries must be int8 codes [nq, dim] and float32 scales [nq]")
         codes, scales = self._use()
-        nq, n = query_codes.shape[0], self._len
+        nq, n = query_codes.shape[0], codes.shape[0]
         most = max(1, self._BLOCK // self._BLOCK_ROWS)
         if nq > most:
             parts = [self.search_codes(query_codes[a:a + most], query_scales[a:a + most], k) for a in range(0, nq, most)]

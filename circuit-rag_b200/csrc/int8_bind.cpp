@@ -31,11 +31,26 @@ namespace {
 using at::Tensor;
 
 struct Refused {
-  PyObject* type;
+  PyObject* type;  // nullptr: NativeLibraryError
   std::string message;
 };
 [[noreturn]] void value_error(std::string m) { throw Refused{PyExc_ValueError, std::move(m)}; }
 [[noreturn]] void runtime_error(std::string m) { throw Refused{PyExc_RuntimeError, std::move(m)}; }
+
+// Lets other Python threads run: an allocation may wait for the device, and a launch behind a thousand pending ones
+// waits for these.  In its scope no Python object is touched (a Refused only names its type).
+struct OtherThreadsRun {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~OtherThreadsRun() { PyEval_RestoreThread(state); }
+};
+
+PyObject* native_error() {  // borrowed: the class lives as long as its module
+  PyObject* module = PyImport_ImportModule("circuit_rag._native");
+  PyObject* type = module ? PyObject_GetAttrString(module, "NativeLibraryError") : nullptr;
+  Py_XDECREF(module);
+  if (!type) PyErr_Clear();
+  return type ? type : PyExc_RuntimeError;
+}
 
 // Sets the Python error of what a call threw; nothing gets past it.
 template <typename F>
@@ -44,7 +59,7 @@ PyObject* guarded(F&& f) {
   try {
     return f();
   } catch (const Refused& r) {
-    PyErr_SetString(r.type, r.message.c_str());
+    PyErr_SetString(r.type ? r.type : native_error(), r.message.c_str());
     return nullptr;
   }
   END_HANDLE_TH_ERRORS
@@ -53,28 +68,18 @@ PyObject* guarded(F&& f) {
 void native(int rc, const char* what) {
   if (!rc) return;
   const char* why = circuit_last_error();
-  std::string m = std::string(what) + " failed (" + std::to_string(rc) + "): " + (why ? why : "");
-  PyObject* module = PyImport_ImportModule("circuit_rag._native");
-  PyObject* type = module ? PyObject_GetAttrString(module, "NativeLibraryError") : nullptr;
-  Py_XDECREF(module);
-  if (!type) PyErr_Clear();
-  throw Refused{type ? type : PyExc_RuntimeError, std::move(m)};  // the class lives as long as its module
+  throw Refused{nullptr, std::string(what) + " failed (" + std::to_string(rc) + "): " + (why ? why : "")};
 }
 
-Tensor given_tensor(PyObject* o, const char* name) {
+Tensor cuda_tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) runtime_error(std::string(name) + " must be CUDA tensor");
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda()) runtime_error(std::string(name) + " must be CUDA tensor");
   return t;
 }
-// A tensor to read: a view that stands for the negative of its memory (the imaginary part of a conjugate) as a copy.
-Tensor cuda_tensor(PyObject* o, const char* name) {
-  Tensor t = given_tensor(o, name);
-  return t.is_neg() ? t.resolve_neg() : t;
-}
 // A tensor to write.
 Tensor cuda_target(PyObject* o, const char* name) {
-  Tensor t = given_tensor(o, name);
+  Tensor t = cuda_tensor(o, name);
   if (t.is_neg()) value_error(std::string(name) + " must not be a view of its negative");
   return t;
 }
@@ -104,14 +109,19 @@ void no_gradient(const Tensor& t, const char* name) {
     runtime_error(std::string(name) + " carries a forward gradient: the 8-bit rows have none (use its primal)");
 }
 
-// A [n, dim] tensor of values that lie next to each other in each row (a copy if they do not).
+// A tensor to read as it lies in memory: a view that stands for its negative (the imaginary part of a conjugate) as a
+// copy, and one whose values do not lie next to each other (in each row).
+Tensor dense(const Tensor& t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+Tensor dense_rows(const Tensor& t) { return !t.is_neg() && plain_rows(t) ? t : dense(t); }
+
+// A [n, dim] tensor of values.
 Tensor value_rows(PyObject* o, const char* name) {
   Tensor t = cuda_tensor(o, name);
   if (t.dim() != 2) value_error(std::string(name) + " must have shape [n, dim]");
   if (type_code(t.scalar_type()) < 0) value_error(std::string(name) + " must be float32, float16 or bfloat16");
   no_gradient(t, name);
   check_dim(t.size(1));
-  return plain_rows(t) ? t : t.contiguous();
+  return t;
 }
 
 Tensor index_tensor(PyObject* o, const char* name, const at::Device& dev) {
@@ -119,7 +129,7 @@ Tensor index_tensor(PyObject* o, const char* name, const at::Device& dev) {
   if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
     value_error(std::string(name) + " must be int32 or int64");
   if (t.device() != dev) value_error(std::string(name) + " must be on the rows' device");
-  return t.contiguous();
+  return t;
 }
 
 void check_pair(const Tensor& codes, const Tensor& scales, const char* name) {
@@ -180,7 +190,7 @@ PyObject* given(PyObject* o) {
 PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
   return guarded([&]() -> PyObject* {
     if (count != 7) value_error("quantize takes 7 arguments");
-    const Tensor rows = value_rows(a[0], "rows");
+    Tensor rows = value_rows(a[0], "rows");
     const at::Device dev = rows.device();
     const c10::cuda::CUDAGuard guard(dev);
     const int64_t n = rows.size(0), dim = rows.size(1);
@@ -201,7 +211,6 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
       if (weight.dim() != 1 || weight.size(0) != dim || weight.device() != dev)
         value_error("weight must have shape [dim] and be on the rows' device");
       no_gradient(weight, "weight");
-      weight = weight.contiguous();
     }
     const bool out = a[6] != Py_None;
     if (a[5] != Py_None) {
@@ -219,28 +228,36 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
       if (codes.device() != dev) value_error("out must be on the rows' device");
       if (codes.size(1) != dim) value_error("out must have the rows' dim");
       if (!slots.defined() && codes.size(0) != n) value_error("out must hold as many rows as there are (or give slots)");
-    } else {
-      codes = fresh_codes(n, dim, dev);
-      scales = fresh({n}, at::kFloat, dev);
     }
-    if (residual.defined()) summed = fresh({n, dim}, rows.scalar_type(), dev);
-    if (n && codes.size(0)) {
-      native(circuit_op_quantize_rows(
-                 rows.const_data_ptr(), type_code(rows.scalar_type()), n, (int)dim, step(rows),
-                 residual.defined() ? residual.const_data_ptr() : nullptr, residual.defined() ? step(residual) : 0,
-                 weight.defined() ? weight.const_data_ptr() : nullptr,
-                 weight.defined() ? type_code(weight.scalar_type()) : 0, (int)norm, (float)eps,
-                 summed.defined() ? summed.mutable_data_ptr() : nullptr, dim,
-                 slots.defined() ? slots.const_data_ptr() : nullptr, slots.defined() ? (int)slots.element_size() : 0,
-                 codes.size(0), codes.mutable_data_ptr<int8_t>(), step(codes), scales.mutable_data_ptr<float>(),
-                 c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
-             "quantize_rows");
-      if (out) {
-        written(codes);
-        written(scales);
+    {
+      const OtherThreadsRun scope;
+      rows = dense_rows(rows);
+      if (residual.defined()) residual = dense_rows(residual);
+      if (weight.defined()) weight = dense(weight);
+      if (slots.defined()) slots = dense(slots);
+      if (!out) {
+        codes = fresh_codes(n, dim, dev);
+        scales = fresh({n}, at::kFloat, dev);
       }
-    } else if (n && summed.defined()) {  // a store without rows: nothing is written, the sum is still due
-      at::add_out(summed, rows, residual);
+      if (residual.defined()) summed = fresh({n, dim}, rows.scalar_type(), dev);
+      if (n && codes.size(0)) {
+        native(circuit_op_quantize_rows(
+                   rows.const_data_ptr(), type_code(rows.scalar_type()), n, (int)dim, step(rows),
+                   residual.defined() ? residual.const_data_ptr() : nullptr, residual.defined() ? step(residual) : 0,
+                   weight.defined() ? weight.const_data_ptr() : nullptr,
+                   weight.defined() ? type_code(weight.scalar_type()) : 0, (int)norm, (float)eps,
+                   summed.defined() ? summed.mutable_data_ptr() : nullptr, dim,
+                   slots.defined() ? slots.const_data_ptr() : nullptr, slots.defined() ? (int)slots.element_size() : 0,
+                   codes.size(0), codes.mutable_data_ptr<int8_t>(), step(codes), scales.mutable_data_ptr<float>(),
+                   c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
+               "quantize_rows");
+        if (out) {
+          written(codes);
+          written(scales);
+        }
+      } else if (n && summed.defined()) {  // a store without rows: nothing is written, the sum is still due
+        at::add_out(summed, rows, residual);
+      }
     }
     PyObject* c = out ? given(PyTuple_GET_ITEM(a[6], 0)) : wrap(codes);
     PyObject* s = out ? given(PyTuple_GET_ITEM(a[6], 1)) : wrap(scales);
@@ -268,8 +285,6 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const at::Device dev = codes.device();
     const c10::cuda::CUDAGuard guard(dev);
     const int64_t rows = codes.size(0), dim = codes.size(1);
-    if (!plain_rows(codes)) codes = codes.contiguous();
-    scales = scales.contiguous();
     Tensor ids, out;
     int64_t n = rows, out_step = dim;
     if (a[2] != Py_None) {
@@ -285,21 +300,28 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
       no_gradient(out, "out");
       check_target(out, "out");
       out_step = step(out);
-    } else if (ids.defined()) {
-      at::DimVector shape(ids.sizes().begin(), ids.sizes().end());
-      shape.push_back(dim);
-      out = fresh(shape, type, dev);
-    } else {
-      out = fresh({n, dim}, type, dev);
     }
-    if (n)
-      native(circuit_op_dequantize_rows(
-                 codes.const_data_ptr<int8_t>(), step(codes), scales.const_data_ptr<float>(), rows, (int)dim,
-                 ids.defined() ? ids.const_data_ptr() : nullptr, ids.defined() ? (int)ids.element_size() : 0, n,
-                 out.mutable_data_ptr(), type_code(type), out_step,
-                 c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
-             "dequantize_rows");
-    if (n && have) written(out);
+    {
+      const OtherThreadsRun scope;
+      if (!have) {
+        at::DimVector shape;
+        if (ids.defined()) shape.append(ids.sizes().begin(), ids.sizes().end());
+        else shape.push_back(n);
+        shape.push_back(dim);
+        out = fresh(shape, type, dev);
+      }
+      codes = dense_rows(codes);
+      scales = dense(scales);
+      if (ids.defined()) ids = dense(ids);
+      if (n)
+        native(circuit_op_dequantize_rows(
+                   codes.const_data_ptr<int8_t>(), step(codes), scales.const_data_ptr<float>(), rows, (int)dim,
+                   ids.defined() ? ids.const_data_ptr() : nullptr, ids.defined() ? (int)ids.element_size() : 0, n,
+                   out.mutable_data_ptr(), type_code(type), out_step,
+                   c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
+               "dequantize_rows");
+      if (n && have) written(out);
+    }
     return have ? given(a[4]) : wrap(out);
   });
 }
@@ -307,7 +329,7 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t count) {
 // Codes as the products read them: rows on 16 bytes, their padding inside the storage (a padded copy if not).
 Tensor code_rows(const Tensor& codes) {
   const int64_t n = codes.size(0), dim = codes.size(1), s = step(codes), p = padded(dim);
-  if ((dim == 1 || codes.stride(1) == 1) && s % 16 == 0 && s >= p &&
+  if (!codes.is_neg() && (dim == 1 || codes.stride(1) == 1) && s % 16 == 0 && s >= p &&
       reinterpret_cast<uintptr_t>(codes.const_data_ptr()) % 16 == 0 &&
       (p == dim || codes.storage_offset() + (n - 1) * s + p <= (int64_t)codes.storage().nbytes()))
     return codes;
@@ -338,7 +360,6 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t count) {
       if (bias.scalar_type() != at::kFloat || bias.dim() != 1 || bias.size(0) != n || bias.device() != dev)
         value_error("bias must be float32 of shape [n] on the rows' device");
       no_gradient(bias, "bias");
-      bias = bias.contiguous();
     }
     int64_t out_step = n;
     const bool have = a[6] != Py_None;
@@ -350,22 +371,28 @@ PyObject* scores(PyObject*, PyObject* const* a, Py_ssize_t count) {
       no_gradient(out, "out");
       check_target(out, "out");
       out_step = step(out);
-    } else {
-      out = fresh_results(nq, n, type, dev);
-      out_step = step(out);
     }
-    if (nq && n) {
-      queries = code_rows(queries);
-      codes = code_rows(codes);
-      query_scales = query_scales.contiguous();
-      row_scales = row_scales.contiguous();
-      native(circuit_op_int8_scores(queries.const_data_ptr<int8_t>(), step(queries), query_scales.const_data_ptr<float>(),
-                                    nq, codes.const_data_ptr<int8_t>(), step(codes), row_scales.const_data_ptr<float>(),
-                                    n, (int)dim, bias.defined() ? bias.const_data_ptr<float>() : nullptr,
-                                    out.mutable_data_ptr(), type_code(type), out_step,
-                                    c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
-             "int8_scores");
-      if (have) written(out);
+    {
+      const OtherThreadsRun scope;
+      if (!have) {
+        out = fresh_results(nq, n, type, dev);
+        out_step = step(out);
+      }
+      if (nq && n) {
+        queries = code_rows(queries);
+        codes = code_rows(codes);
+        query_scales = dense(query_scales);
+        row_scales = dense(row_scales);
+        if (bias.defined()) bias = dense(bias);
+        native(circuit_op_int8_scores(queries.const_data_ptr<int8_t>(), step(queries),
+                                      query_scales.const_data_ptr<float>(), nq, codes.const_data_ptr<int8_t>(),
+                                      step(codes), row_scales.const_data_ptr<float>(), n, (int)dim,
+                                      bias.defined() ? bias.const_data_ptr<float>() : nullptr, out.mutable_data_ptr(),
+                                      type_code(type), out_step,
+                                      c10::cuda::getCurrentCUDAStream(dev.index()).stream()),
+               "int8_scores");
+        if (have) written(out);
+      }
     }
     return have ? given(a[6]) : wrap(out);
   });

@@ -1,4 +1,7 @@
 """8-bit rows on the GPU: the calls at the edge of what the documents allow."""
+import threading
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -97,8 +100,8 @@ def test_growth_keeps_memory_that_another_stream_reads():
     x = _rows(n, d, 1)
     store.append(x)
     want = store.scores(x[:3])
-    old = store._codes.data_ptr(), store._scales.data_ptr()
-    size = store._codes.shape
+    old = store._made[0].data_ptr(), store._made[1].data_ptr()
+    size = store._made[0].shape
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -277,3 +280,69 @@ def test_status_waits_for_its_stream_only():
     assert not torch.cuda.default_stream().query()
     int8.check_products()
     assert torch.cuda.default_stream().query()
+
+
+@pytest.mark.parametrize("call", ["quantize", "dequantize", "scores"])
+def test_other_threads_run_while_a_launch_waits(call):
+    """Behind about a thousand pending launches a further one waits: other Python threads go on meanwhile."""
+    x = _rows(4, 32)
+    codes, scales = quantize_rows(x)
+    out, products = torch.empty(4, 32, device=DEV), torch.empty(4, 4, device=DEV)
+    todo = {"quantize": lambda: quantize_rows(x, out=(codes, scales)), "dequantize": lambda: dequantize_rows(codes, scales, out=out),
+            "scores": lambda: int8_scores(codes, scales, codes, scales, out=products)}[call]
+    todo()
+    torch.cuda.synchronize()
+    gaps, stop = [0.0], threading.Event()
+
+    def tick():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            gaps[0], last = max(gaps[0], now - last), now
+
+    thread = threading.Thread(target=tick)
+    thread.start()
+    try:
+        time.sleep(0.05)
+        gaps[0] = 0.0
+        longest = 0.0
+        torch.cuda._sleep(1_500_000_000)  # about three quarters of a second
+        for _ in range(3000):
+            start = time.perf_counter()
+            todo()
+            longest = max(longest, time.perf_counter() - start)
+        torch.cuda.synchronize()
+    finally:
+        stop.set()
+        thread.join()
+    assert longest < 0.2 or gaps[0] < longest / 2, (longest, gaps[0])
+
+
+def test_a_thread_searches_while_another_appends():
+    store = Int8Rows(0, 64, DEV)
+    x = _rows(30000, 64, 1)
+    store.append(x[:50])
+    torch.cuda.synchronize()
+    failed, stop = [], threading.Event()
+
+    def search():
+        try:
+            q = x[:3].clone()
+            while not stop.is_set():
+                scores, ids = store.search(q, 3)
+                if ids[:, 0].tolist() != [0, 1, 2]:
+                    failed.append(ids)
+        except Exception as e:  # shown by the main thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=search) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for a in range(50, 30000, 599):
+        store.append(x[a:a + 599])
+    stop.set()
+    for t in threads:
+        t.join()
+    assert not failed, failed[0]
+    assert torch.equal(store.scales, quantize_rows(x)[1])

@@ -18,9 +18,9 @@ def _one_stream(monkeypatch):
 def _host_store(places, dim=8):
     """A store whose buffers lie on the CPU, every place taken (scale 1 + place)."""
     store = Int8Rows.__new__(Int8Rows)
-    store._in_graph, store._captured, store._made_on = False, [], 1
+    store._in_graph, store._captured = False, []
     store.device, store.dim, store._len = torch.device("cpu"), dim, places
-    store._codes, store._scales = store._buffers(places)
+    store._made = *store._buffers(places), 1
     store.scales.copy_(torch.arange(places) + 1.0)
     return store
 
@@ -54,7 +54,7 @@ def test_remove_with_places_in_reserve():
     store = _host_store(5)
     store._len = 3
     store.remove(torch.tensor([3, 4]))
-    assert store._scales[3:5].tolist() == [4.0, 5.0]
+    assert store._made[1][3:5].tolist() == [4.0, 5.0]
 
 
 @pytest.mark.parametrize("slots", [torch.tensor([True, False, True]), torch.tensor([0.5]), [0], 0, None])
@@ -68,7 +68,7 @@ def test_remove_refuses_what_is_no_place(slots):
 def _search(store, products, query_scales, k, monkeypatch):
     """search_codes with given products, as if the kernel had written them."""
     def fake(qc, qs, codes, scales, **kw):
-        a = (codes.data_ptr() - store._codes.data_ptr()) // store._codes.shape[1]
+        a = (codes.data_ptr() - store._made[0].data_ptr()) // store._made[0].shape[1]
         return products[:, a:a + codes.shape[0]].clone()
 
     monkeypatch.setattr(int8, "int8_scores", fake)
@@ -175,18 +175,18 @@ CALLS = {
 def test_memory_is_kept_for_the_streams_that_use_it(call, monkeypatch):
     """Growth drops the old buffers: the allocator knows every stream that may still read or write them."""
     store = _host_store(4)
-    buffers = {store._codes.data_ptr(), store._scales.data_ptr()}
+    buffers = {store._made[0].data_ptr(), store._made[1].data_ptr()}
     now, log = _streams(store, monkeypatch)
     CALLS[call](store)
     assert log == []  # its own stream: the allocator orders that by itself
     store = _host_store(4)
-    buffers = {store._codes.data_ptr(), store._scales.data_ptr()}
+    buffers = {store._made[0].data_ptr(), store._made[1].data_ptr()}
     now, log = _streams(store, monkeypatch)
     now[0] = 5
     CALLS[call](store)
     assert {b for b, s in log} == buffers and {s for b, s in log} == {5}
     if call == "append":
-        assert store._made_on == 5 and len(store) == 13
+        assert store._made[2] == 5 and len(store) == 13
 
 
 def test_buffers_of_a_captured_call_outlive_growth(monkeypatch):
@@ -197,7 +197,7 @@ def test_buffers_of_a_captured_call_outlive_growth(monkeypatch):
     with pytest.raises(RuntimeError):
         CALLS["append"](store)  # would copy the rows of now at every replay
     assert len(store) == 4
-    old = store._codes
+    old = store._made[0]
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     CALLS["append"](store)
     assert len(store) == 13 and store._captured[0][0] is old
