@@ -105,7 +105,7 @@ def test_growth_keeps_memory_that_another_stream_reads():
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        torch.cuda._sleep(1_000_000_000)  # about half a second
         got = store.scores(x[:3])
     assert store.append(x[:1]) == range(n, n + 1)  # the buffers are full: new ones
     taken = [torch.full(size, 99, dtype=torch.int8, device=DEV) for _ in range(3)]
@@ -274,7 +274,7 @@ def test_feedback_does_not_depend_on_the_length_of_the_query():
 def test_status_waits_for_its_stream_only():
     side = torch.cuda.Stream()
     torch.cuda.synchronize()
-    torch.cuda._sleep(400_000_000)  # about a fifth of a second on the default stream
+    torch.cuda._sleep(1_000_000_000)  # about half a second on the default stream
     with torch.cuda.stream(side):
         int8.check_products()
     assert not torch.cuda.default_stream().query()
