@@ -2,12 +2,12 @@
 a store of such rows, and the products of queries with them.
 
 A row of ``dim`` values is kept as ``dim`` int8 codes and one float32 scale: a quarter of the bytes of the float32 rows
-that a CircuitIndex scans.  The products are exact sums of the codes, so they equal the inner products of the rows as
-stored; against the original rows each value is off by at most half a code (scale / 2).
+that a CircuitIndex scans.  The products sum the codes exactly, so up to the roundings of the scales they are the inner
+products of the rows as stored; against the original rows each value is off by at most half a code (scale / 2).
 
 The calls run on the current torch stream of their tensors' device, never synchronise, and may be captured into a CUDA
-graph.  They serve only: there is no backward pass, and rows that ask for a gradient are refused.  No reference
-counterpart (the reference keeps float32 rows only).
+graph.  They serve only: there is no backward pass, and tensors that ask for a gradient or carry a forward one are
+refused.  Given results count as written in place.  No reference counterpart (the reference keeps float32 rows only).
 """
 from typing import Optional, Tuple
 
@@ -56,7 +56,8 @@ def rms_norm_quantize(rows: torch.Tensor, residual: Optional[torch.Tensor] = Non
 
     v = rows + residual, rounded once to the rows' type and returned as ``summed`` (None without a residual); the codes
     and scales are those of v / sqrt(mean(v^2) + eps) * weight (weight of the rows' type or float32, or none).  The
-    sum of squares is held in 32 bits and cancels in the codes.  ``slots`` and ``out`` as in quantize_rows."""
+    sum of squares is held in 32 bits and cancels in the codes.  A row with an infinity, a NaN, or a product with its
+    weight beyond float32 gets codes 0 and scale NaN.  ``slots`` and ``out`` as in quantize_rows."""
     return _bind().quantize(rows, residual, weight, _native.CIRCUIT_NORM_RMS, eps, slots, out)
 
 
@@ -72,9 +73,11 @@ def int8_scores(query_codes: torch.Tensor, query_scales: torch.Tensor, codes: to
                 bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float32,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Products [nq, n] of 8-bit queries with 8-bit rows: query_scales[i] * scales[j] * (codes' inner product), plus
-    bias[j] (float32 [n]: a prior of each row, or -|x|^2 / 2 for distances), rounded once to ``dtype``.
+    bias[j] (float32 [n]: a prior of each row, or -|x|^2 / 2 for distances).
 
-    The sum over dim is exact; times the query's scale it has to stay in the range of float32 (values up to 1e32).  A
+    The sum over dim is exact.  It is converted to float32 (a rounding beyond 2^24, which takes more than 1,040 values),
+    multiplied with the query's scale (a rounding; the product has to stay in the range: values up to 1e32), multiplied
+    with the row's and added to the bias in one operation (a rounding), and rounded to ``dtype``.  A
     new result of 256 rows and more starts its rows on 128 bytes (its row stride is n rounded up, so it is only
     contiguous where n allows); ``out`` may have any row stride.  Codes whose rows do not start on 16 bytes or end
     without padding are copied first; those of quantize_rows and Int8Rows never are."""

@@ -123,8 +123,9 @@ int circuit_op_dequantize_rows(const int8_t* codes, int64_t code_stride, const f
                                const void* ids, int id_bytes, int64_t n, void* out, int dtype, int64_t out_stride,
                                void* stream);
 
-/* out[i][j] = query_scales[i] * scales[j] * sum_k queries[i][k] codes[j][k] (+ bias[j]), rounded once to dtype; the
- * sum is exact (32-bit integers), and times the query's scale it has to stay in the range of fp32.  Code rows start on
+/* out[i][j] = query_scales[i] * scales[j] * sum_k queries[i][k] codes[j][k] (+ bias[j]).  The sum is exact (32-bit
+ * integers); as fp32 it is multiplied with the query's scale (the product has to stay in the range), then with the row's
+ * and added to the bias in one operation: up to three fp32 roundings, and one to dtype.  Code rows start on
  * 16 bytes and their strides are multiples of 16; up to 15 bytes past dim are read in each row (the last one's too)
  * and do not count. */
 int circuit_op_int8_scores(const int8_t* queries, int64_t query_stride, const float* query_scales, int64_t num_queries,
