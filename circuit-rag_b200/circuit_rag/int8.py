@@ -126,6 +126,10 @@ class Int8Rows:
         # one scale more than places: what is meant for no place goes there
         return codes, torch.full((n + 1,), float("nan"), dtype=torch.float32, device=self.device)
 
+    def __setstate__(self, state):  # a copy: its buffers are new ones of the current stream, and no graph has them
+        self.__dict__.update(state, _in_graph=False, _captured=[])
+        self._made = *self._made[:2], _stream(self.device)
+
     def _use(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """Codes and scales for the current stream: their memory is kept for it when a growing store drops them."""
         n, now = self._len, _stream(self.device)  # the length first: later buffers hold as many places

@@ -1,4 +1,6 @@
 """8-bit rows on the GPU: the calls at the edge of what the documents allow."""
+import copy
+import pickle
 import threading
 import time
 
@@ -346,3 +348,21 @@ def test_a_thread_searches_while_another_appends():
         t.join()
     assert not failed, failed[0]
     assert torch.equal(store.scales, quantize_rows(x)[1])
+
+
+def test_a_copy_of_a_store_is_its_own():
+    store = Int8Rows(0, 24, DEV)
+    x = _rows(10, 24, 1)
+    store.append(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        copies = [copy.deepcopy(store), pickle.loads(pickle.dumps(store))]
+        for other in copies:
+            assert other._made[2] == side.cuda_stream  # its memory is this stream's
+            other.append(x)
+    side.synchronize()
+    store.remove(torch.tensor([3], device=DEV))
+    for other in copies:
+        assert len(other) == 20 and len(store) == 10
+        assert torch.equal(other.scales, quantize_rows(x)[1].repeat(2))
